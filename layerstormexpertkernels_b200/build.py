@@ -37,7 +37,7 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["common.cu", "gating.cu", "permute.cu", "swiglu.cu", "grouped_gemm.cu",
               "layer.cu", "ep.cu"]
-HEADERS = ["common.cuh", "swiglu.cuh"]
+HEADERS = ["common.cuh", "swiglu.cuh", "ep_peer.cuh", "umma.cuh"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = GENCODE + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
                         "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
