@@ -262,6 +262,77 @@ LSEK_API lsek_status lsek_grouped_gemm_swiglu_bf16(void* Hout, const void* A,
                                           float swiglu_limit, void* workspace,
                                           size_t workspace_bytes, void* stream);
 
+/* ---- NVFP4: 4-bit experts -------------------------------------------------- */
+/* An NVFP4 tensor of rows of K elements is
+ *   codes  [rows, K/2] uint8: two E2M1 codes a byte, the even element in the
+ *          low nibble (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 is the sign)
+ *   scales [rows, K/16] E4M3: one for 16 consecutive elements of a row
+ *   global_scale: one float32 (per expert for weights), NULL for 1
+ * and stands for code * scale * global_scale.  codes and scales are those of
+ * ref_nvfp4_dequant (tests/test_reference.py:19-53); the reference's kernels
+ * for the format are in a separate library.  The GEMMs take the scales of
+ * their weights in tiles: [E, tiles, K/64, 512] bytes, tile t of an expert
+ * holding rows 128 t .. 128 t + 127 and, for each 64 elements of K, the four
+ * scales of row r at byte 16 * (r % 32) + 4 * (r / 32); rows past the last
+ * are zero.  The gate and the up rows of a gate/up tensor are tiled apart
+ * (2 * ceil(I / 128) tiles an expert). */
+
+/* Quantises x (bf16 or fp16: dtype) of `groups` groups of `rows` rows of k
+ * elements, contiguous, with one global scale per group.  For each block of
+ * 16 elements, every operation rounded to float32 once:
+ *   scale = e4m3(amax / (6 * global_scale))       saturating at 448
+ *   code  = e2m1(x * (1 / (scale * global_scale))) saturating at 6
+ * (nearest, halves to even; codes 0 where the scale is 0).  A block that
+ * holds an infinity or a NaN gets the scale NaN.  k % 16 == 0; global scales
+ * are positive, in [2^-100, 2^100]; codes 8-byte aligned. */
+LSEK_API lsek_status lsek_nvfp4_quantize(void* codes, void* scales, const void* x,
+                                const float* global_scale, int64_t groups, int64_t rows,
+                                int32_t k, int32_t dtype, void* stream);
+
+/* The values: out = code * scale * global_scale in float32, rounded to dtype
+ * (bf16, fp16 or fp32).  out 16-byte, codes 8-byte aligned. */
+LSEK_API lsek_status lsek_nvfp4_dequantize(void* out, const void* codes, const void* scales,
+                                  const float* global_scale, int64_t groups, int64_t rows,
+                                  int32_t k, int32_t dtype, void* stream);
+
+/* lsek_moe_permute with the rows quantised on the way: each token of
+ * hidden_states [T, H] bf16 is read and quantised once (as by
+ * lsek_nvfp4_quantize with one global scale) and stored to its topk rows of
+ * codes [T*topk, H/2] and scales [T*topk, H/16].  The maps are those of
+ * lsek_moe_route.  hidden_dim % 16 == 0. */
+LSEK_API lsek_status lsek_moe_permute_nvfp4(void* codes, void* scales, int32_t* expert_offsets,
+                                   int32_t* src_to_dest_map, int32_t* permuted_idx,
+                                   const void* hidden_states, const int32_t* topk_indices,
+                                   const float* global_scale, int32_t num_tokens, int32_t topk,
+                                   int32_t hidden_dim, int32_t num_experts, void* stream);
+
+/* lsek_grouped_gemm_bf16 on NVFP4 operands: A [rows, K] with row scales, B
+ * [E, N, K] with tiled scales, D [rows, N] bf16 = the fp32 sum of the
+ * products times a_global_scale * b_global_scale[e], rounded once.
+ * K % 64 == 0, N % 32 == 0, tensors 16-byte aligned; expert_offsets and
+ * workspace as there. */
+LSEK_API lsek_status lsek_grouped_gemm_nvfp4(void* D, const void* A, const void* a_scales,
+                                    const void* B, const void* b_scale_tiles,
+                                    const int32_t* expert_offsets, const float* a_global_scale,
+                                    const float* b_global_scale, int32_t num_experts,
+                                    int32_t rows, int32_t N, int32_t K, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Gate/up product, SwiGLU and quantisation in one kernel: equal bit for bit to
+ * lsek_grouped_gemm_nvfp4, lsek_fused_swiglu and lsek_nvfp4_quantize (with
+ * h_global_scale) in a row.  W_gu [E, 2I, K]; h_codes [rows, I/2], h_scales
+ * [rows, I/16].  K % 64 == 0, I % 32 == 0, tensors 16-byte aligned. */
+LSEK_API lsek_status lsek_grouped_gemm_swiglu_nvfp4(void* h_codes, void* h_scales, const void* A,
+                                           const void* a_scales, const void* W_gu,
+                                           const void* gu_scale_tiles,
+                                           const int32_t* expert_offsets,
+                                           const float* a_global_scale,
+                                           const float* gu_global_scale,
+                                           const float* h_global_scale, int32_t num_experts,
+                                           int32_t rows, int32_t I, int32_t K,
+                                           float swiglu_limit, void* workspace,
+                                           size_t workspace_bytes, void* stream);
+
 /* ---- expert-parallel dispatch / combine ----------------------------------- */
 /* Experts are sharded over world_size ranks, rank g owning experts
  * [g*E/G, (g+1)*E/G).  These kernels prepare and consume the two all-to-all
@@ -483,6 +554,28 @@ LSEK_API lsek_status lsek_moe_layer_forward(
     const void* W_gu, const void* W_down, const lsek_topk_gating_params* gp,
     int32_t hidden_dim, int32_t inter_dim, float swiglu_limit,
     float* topk_weights, int32_t* topk_indices, void* workspace,
+    size_t workspace_bytes, void* const* stage_events, void* stream);
+
+/* Scratch bytes for lsek_moe_layer_forward_nvfp4. */
+LSEK_API size_t lsek_moe_layer_nvfp4_workspace_size(int32_t num_tokens, int32_t hidden_dim,
+                                           int32_t inter_dim, int32_t num_experts,
+                                           int32_t topk);
+
+/* lsek_moe_layer_forward on NVFP4 experts:
+ *   topk_gating -> route -> quantising permute -> gate/up GEMM + SwiGLU +
+ *   quantisation -> down GEMM -> weighted unpermute,
+ * the same stages for stage_events.  W_gu [E, 2I, H] and W_down [E, H, I] with
+ * tiled scales and global scales [E]; hidden_global_scale and
+ * inter_global_scale are one float32 each on the device, NULL for 1.
+ * hidden_dim and inter_dim % 64 == 0.  out equals the stages' entry points in
+ * a row, bit for bit. */
+LSEK_API lsek_status lsek_moe_layer_forward_nvfp4(
+    void* out, const void* hidden, const float* logits, const float* bias, const void* W_gu,
+    const void* gu_scale_tiles, const float* gu_global_scale, const void* W_down,
+    const void* down_scale_tiles, const float* down_global_scale,
+    const float* hidden_global_scale, const float* inter_global_scale,
+    const lsek_topk_gating_params* gp, int32_t hidden_dim, int32_t inter_dim,
+    float swiglu_limit, float* topk_weights, int32_t* topk_indices, void* workspace,
     size_t workspace_bytes, void* const* stage_events, void* stream);
 
 #ifdef __cplusplus

@@ -34,21 +34,30 @@ from ._C import (  # noqa: E402,F401
     device_error,
     fused_swiglu,
     grouped_gemm_bf16,
+    grouped_gemm_nvfp4,
     grouped_gemm_swiglu_bf16,
+    grouped_gemm_swiglu_nvfp4,
     moe_combine_reduce_slots_bf16_to_bf16,
     moe_combine_reduce_slots_fp32_to_bf16,
+    moe_layer_forward_nvfp4_out,
     moe_layer_forward_out,
+    moe_layer_nvfp4_workspace_size,
     moe_layer_workspace_size,
     moe_permute,
+    moe_permute_nvfp4,
     moe_route,
     moe_unpermute,
     moe_unpermute_bf16_perslot,
     moe_unpermute_fp32,
+    nvfp4_dequantize,
+    nvfp4_quantize,
     topk_gating,
     version,
 )
 from .layer import (STAGES, HostPipeline, MoELayer, StageEvents, bind_host_to_device,  # noqa: E402,F401
                     moe_layer_forward)
+from .nvfp4 import (MoELayerNVFP4, moe_layer_forward_nvfp4, nvfp4_quantize_weights,  # noqa: E402,F401
+                    nvfp4_tile_scales)
 
 __all__ = [
     "adaptive_gating", "device_error", "fused_swiglu", "grouped_gemm_bf16",
@@ -57,5 +66,9 @@ __all__ = [
     "moe_layer_workspace_size", "moe_permute", "moe_route", "moe_unpermute", "moe_unpermute_bf16_perslot",
     "moe_unpermute_fp32", "topk_gating", "version", "MoELayer", "HostPipeline", "StageEvents", "bind_host_to_device",
     "STAGES",
+    "grouped_gemm_nvfp4", "grouped_gemm_swiglu_nvfp4", "moe_layer_forward_nvfp4",
+    "moe_layer_forward_nvfp4_out", "moe_layer_nvfp4_workspace_size", "moe_permute_nvfp4",
+    "nvfp4_dequantize", "nvfp4_quantize", "nvfp4_quantize_weights", "nvfp4_tile_scales",
+    "MoELayerNVFP4",
     "LIBRARY_PATH",
 ]

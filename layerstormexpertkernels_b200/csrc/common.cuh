@@ -55,7 +55,8 @@ cudaError_t once_per_device(PerDeviceOnce& once, F&& f) {
 
 // Codes a kernel records when its bounded wait expires; read back (and
 // cleared) by lsek_device_error.  Each translation unit with waiting kernels
-// keeps its own word (grouped_gemm.cu, ep.cu); lsek_device_error reads both.
+// keeps its own word (grouped_gemm.cu, nvfp4_gemm.cu, ep.cu); lsek_device_error
+// reads them all.
 enum DeviceError : int32_t {
   kDevErrNone = 0,
   kDevErrGemmProducerWait = 1,
@@ -63,6 +64,7 @@ enum DeviceError : int32_t {
   kDevErrGemmEpilogueWait = 3,
   kDevErrEpDispatchWait = 4,   // a peer's dispatch rows did not arrive in time
   kDevErrEpCombineWait = 5,    // a peer's combine slots did not arrive in time
+  kDevErrGemmScaleWait = 6,    // the NVFP4 GEMM's scale warps
 };
 
 // Nanoseconds since an arbitrary epoch (globaltimer); used to bound waits.

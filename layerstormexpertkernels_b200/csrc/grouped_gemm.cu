@@ -82,7 +82,8 @@
 
 namespace lsek {
 
-lsek_status ep_take_device_error(int32_t* code);  // ep.cu
+lsek_status ep_take_device_error(int32_t* code);   // ep.cu
+lsek_status fp4_take_device_error(int32_t* code);  // nvfp4_gemm.cu
 
 EncodeTiledFn tensor_map_encoder() {
   static EncodeTiledFn fn = nullptr;
@@ -1036,7 +1037,10 @@ extern "C" lsek_status lsek_device_error(int32_t* code, void* stream) {
   int32_t ep_code = 0;
   const lsek_status s = ep_take_device_error(&ep_code);
   if (s != LSEK_OK) return s;
-  if (*code == 0) *code = ep_code;
+  int32_t fp4_code = 0;
+  const lsek_status f = fp4_take_device_error(&fp4_code);
+  if (f != LSEK_OK) return f;
+  if (*code == 0) *code = ep_code != 0 ? ep_code : fp4_code;
   return LSEK_OK;
 }
 

@@ -1,0 +1,781 @@
+// Grouped NVFP4 expert GEMM on the block-scaled 4-bit path of the
+// 5th-generation tensor cores (tcgen05 kind::mxf4nvf4).
+//
+// Problem: for every expert e and every row r of it
+//   D[r, n] = bf16(ga * gb[e] * sum_k (a[r,k] sa[r,k/16]) (b[e,n,k] sb[e,n,k/16]))
+// with E2M1 codes a, b (two per byte), E4M3 scales sa, sb for 16 elements
+// along K, and float32 global scales ga (activations) and gb[e] (weights).
+// The tensor core multiplies code * scale products exactly and sums them in
+// fp32; the epilogue applies the global scales in fp32 and rounds once.
+// SWIGLU mode computes g and u of 128 output columns, rounds both to bf16,
+// applies swiglu_f32, rounds h to bf16 and quantises it (nvfp4.cuh) with the
+// output's global scale: bit for bit the plain GEMM, fused_swiglu and
+// nvfp4_quantize in a row, without their passes over memory.
+//
+// Tiling.  The weights are the MMA's M operand (two boxes of 128 rows), the
+// tokens its N operand (up to kTokRows, rounded up to 16): a tile's cost then
+// follows its token count, and a weight row passes through shared memory once
+// for every chunk of tokens.  An expert's rows are cut into equal chunks of at
+// most kTokRows.  Units are (expert, n-tile, chunk), chunk fastest, so chunks
+// that share a weight tile are taken at about the same time by neighbouring
+// CTAs and the weight tile comes from HBM once.  A persistent grid of one CTA
+// per SM takes units from an atomic counter in caller scratch, or with a
+// static stride where there is none.
+//
+// K runs in stages of 256 elements: one 128-byte swizzled row of codes, four
+// MMAs of K=64, and 16 scale bytes a row.  The MMA reads scales from TMEM,
+// where a 128-row tile of the four scales of one MMA is 32 lanes x 4 columns
+// (row r in lane r % 32, column r / 32), copied there by tcgen05.cp from a
+// 512-byte image in shared memory.  The weight scales lie in global memory in
+// that order already (they are laid out once) and arrive by bulk copies; the
+// activation scales are plain rows [rows, K/16], which start at any expert
+// boundary, and are turned into the image by the scale warps.
+//
+// One CTA = 10 warps and one more for each stage:
+//   warp 0       TMA producer (codes of both operands, weight scales)
+//   warp 1       MMA issuer: tcgen05.cp of a stage's scales into one of two
+//                TMEM buffers, then 4 x 2 MMAs
+//   warps 2-9    epilogue, two groups of four (warp w reads TMEM lanes
+//                32*(w%4)..+31 = its 32 weight rows; the groups alternate
+//                chunks of 16 tokens); each warp turns its 16 x 32 piece in
+//                shared memory so that a lane holds 16 consecutive outputs of
+//                one token: one 32-byte bf16 store, or one NVFP4 block
+//   warps 10-    activation scales, one warp for each ring slot: a warp that
+//                served several slots would not see every phase of their
+//                barriers, and a parity wait tells only neighbouring phases apart
+//
+// TMEM: columns 0..383 hold the accumulators (a unit of up to 96 token
+// columns takes half of them, so its epilogue overlaps the next unit's main
+// loop), 384..511 two buffers of scales (weights 2 boxes x 4 MMAs x 4 columns,
+// tokens 4 x 8).  A buffer is overwritten only after the MMAs that read it
+// have completed (the empty barrier of two stages before).
+//
+// Waits are bounded as in grouped_gemm.cu.
+#include <initializer_list>
+
+#include "nvfp4.cuh"
+#include "swiglu.cuh"
+#include "umma.cuh"
+
+namespace lsek {
+namespace fp4 {
+
+constexpr int kStepK = 64;                        // K of one MMA
+constexpr int kSteps = 4;                         // MMAs (per box) of a stage
+constexpr int kRowBytes = kSteps * kStepK / 2;    // 128: one swizzle row
+constexpr int kBoxRows = 128;                     // weight rows of a box = MMA M
+constexpr int kBoxBytes = kBoxRows * kRowBytes;   // 16 KB
+constexpr int kSfTile = 512;                      // scales of 128 rows for one MMA
+constexpr int kSfBoxBytes = kSteps * kSfTile;     // 2 KB
+constexpr int kEpiWarps = 8;
+constexpr int kFirstSfWarp = 2 + kEpiWarps;
+constexpr int kUnitQ = 4;                         // unit ids in flight between warps
+constexpr int kMaxExperts = 1024;
+constexpr int kAccCols = 192;                     // TMEM columns of an accumulator slot
+constexpr int kSfCol = 2 * kAccCols;              // first column of the scale buffers
+constexpr int kSfBufCols = 64;
+constexpr int kTmemCols = 512;
+constexpr int kStagePitch = 80;                   // epilogue: bytes of a token's 32 bf16 (+ pad)
+
+// TOK: most token rows of a unit; MAX_E: experts that the unit table holds.
+template <int TOK, int STAGES, int MAX_E>
+struct Geom {
+  static constexpr int kTok = TOK;
+  static constexpr int kStages = STAGES;
+  static constexpr int kWarps = kFirstSfWarp + STAGES;  // a scale warp per ring slot
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kMaxE = MAX_E;
+  static constexpr int kHalves = (TOK + 127) / 128;  // scale tiles of the tokens
+  static constexpr int kTokBytes = TOK * kRowBytes;
+  static constexpr int kSfTokBytes = kSteps * kHalves * kSfTile;
+  static constexpr int kStageBytes = 2 * kBoxBytes + kTokBytes + 2 * kSfBoxBytes + kSfTokBytes;
+  static_assert(TOK % 16 == 0 && TOK <= kAccCols, "a unit's tokens fit an accumulator slot");
+  static_assert(kTokBytes % 1024 == 0 && kStageBytes % 1024 == 0, "swizzled boxes on 1 KB");
+};
+using GeomFull = Geom<192, 3, kMaxExperts>;
+// Every expert has at most 32 rows (decode): five stages in flight.
+using GeomDecode = Geom<32, 5, 256>;
+
+template <class G>
+struct SmemT {
+  uint8_t ring[G::kStages][G::kStageBytes];  // 1024-byte aligned
+  uint8_t turn[kEpiWarps][16 * kStagePitch];
+  uint64_t full_bar[G::kStages];   // TMA bytes + the scale warp
+  uint64_t empty_bar[G::kStages];
+  uint64_t acc_full_bar[2];
+  uint64_t acc_empty_bar[2];
+  uint64_t mma_done_bar;
+  uint64_t q_full[kUnitQ];
+  uint64_t q_empty[kUnitQ];
+  int32_t unit_q[kUnitQ];
+  uint32_t tmem_base;
+  int32_t abort;
+  int32_t warp_tot[G::kWarps];
+  int32_t offs[G::kMaxE + 1];
+  int32_t cum[G::kMaxE + 1];
+};
+template <class G>
+constexpr size_t smem_bytes() {
+  return sizeof(SmemT<G>) + 1024;
+}
+static_assert(smem_bytes<GeomFull>() <= 227 * 1024, "shared memory budget");
+static_assert(smem_bytes<GeomDecode>() <= 227 * 1024, "shared memory budget");
+
+struct Params {
+  const int32_t* offsets;  // [E+1]
+  int num_experts;
+  int rows;                // rows of A and of the output
+  int steps;               // K / 64
+  int n_tiles;             // n-tiles per expert
+  int b_rows;              // weight rows per expert
+  int b_tile_rows;         // first-box row step per n-tile
+  int b_second;            // row offset of the second box
+  int sf_tiles;            // 128-row scale tiles per expert
+  int sf_tile_step;        // tile step per n-tile of the first box
+  int sf_second;           // tile offset of the second box
+  const uint8_t* a_sf;     // [rows, K/16]
+  const uint8_t* b_sf;     // [E, sf_tiles, steps, 512]
+  const float* a_global;   // one value, or null: 1
+  const float* b_global;   // [E], or null: 1
+  const float* out_global; // SWIGLU: the output's global scale, or null: 1
+  __nv_bfloat16* D;        // plain: [rows, n_out]
+  uint8_t* out_codes;      // SWIGLU: [rows, n_out/2]
+  uint8_t* out_sf;         // SWIGLU: [rows, n_out/16]
+  int out_tile_cols;       // output columns per tile
+  int n_out;
+  float swiglu_limit;
+  int32_t* counter;        // zeroed unit counter, or null (static stride)
+  int wide_scales;         // rows of a_sf are multiples of 16 bytes (K % 256 == 0)
+};
+
+// ---- PTX ----------------------------------------------------------------------
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+// 512 bytes of shared memory (32 rows of 16 bytes) -> 4 TMEM columns of 32
+// lanes, repeated in the four lane quarters.
+__device__ __forceinline__ void tmem_copy_sf(uint32_t taddr, uint32_t saddr) {
+  // no swizzle; 8-row groups 128 bytes apart, version 1 (sm_100)
+  const uint64_t desc = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) |
+                        (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                         uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor: A and B E2M1 (1 in bits 7-9 and 10-11), scales E4M3
+// (bit 23 = 0), N >> 3 in bits 17-22, M >> 7 in bits 27-28, scale ids 0, K = 64.
+__device__ __forceinline__ uint32_t fp4_idesc(int nn) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(nn >> 3) << 17) |
+         (static_cast<uint32_t>(kBoxRows >> 7) << 27);
+}
+
+// ---- work units -----------------------------------------------------------------
+
+template <class G, class S>
+__device__ __forceinline__ int chunks_of(const S& s, int e) {
+  const int n = s.offs[e + 1] - s.offs[e];
+  return n > 0 ? (n + G::kTok - 1) / G::kTok : 0;
+}
+
+// n-tile n of expert e against `rows` tokens from row0 on.
+struct Unit {
+  int e, n, row0, rows;
+};
+
+// The largest e with cum[e] <= id is the (non-empty) expert that owns the
+// unit; its units are ordered (n-tile, chunk), the chunk fastest.  The chunks
+// are equal up to the rounding to 16 rows.
+template <class G, class S>
+__device__ __forceinline__ Unit decode_unit(const S& s, int num_experts, int id) {
+  int lo = 0, hi = num_experts - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.cum[mid] <= id) lo = mid;
+    else hi = mid - 1;
+  }
+  Unit u;
+  u.e = lo;
+  const int local = id - s.cum[lo];
+  const int c = chunks_of<G>(s, lo);
+  u.n = local / c;
+  const int m = local - u.n * c;
+  const int n = s.offs[lo + 1] - s.offs[lo];
+  const int per = ((n + c - 1) / c + 15) & ~15;
+  u.row0 = s.offs[lo] + m * per;
+  u.rows = min(per, n - m * per);
+  return u;
+}
+
+template <bool SWIGLU, class G>
+__global__ void __launch_bounds__(G::kThreads, 1)
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a64,
+                    const __grid_constant__ CUtensorMap tmap_a16,
+                    const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p) {
+  using Smem = SmemT<G>;
+  constexpr int S = G::kStages;
+  constexpr int kThreads = G::kThreads;
+  constexpr int kTokOff = 2 * kBoxBytes;
+  constexpr int kSfBOff = kTokOff + G::kTokBytes;       // weight scales
+  constexpr int kSfAOff = kSfBOff + 2 * kSfBoxBytes;    // token scales: tile (step, half)
+  extern __shared__ uint8_t smem_raw[];
+  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                     ~static_cast<uintptr_t>(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int E = p.num_experts;
+
+  // ---- unit table: cum[e] = sum over e' < e of chunks(e') * n_tiles -------------
+  // Offsets are clamped to [0, rows]; an expert whose end precedes its start has
+  // no units, so every stored row stays inside the output.
+  for (int i = tid; i <= E; i += kThreads) {
+    int v = __ldg(p.offsets + i);
+    v = v < 0 ? 0 : (v > p.rows ? p.rows : v);
+    s.offs[i] = v;
+  }
+  if (tid == 0) s.abort = 0;
+  __syncthreads();
+  {
+    const int per = (E + kThreads - 1) / kThreads;
+    const int eb = min(E, tid * per);
+    const int ee = min(E, eb + per);
+    int local = 0;
+    for (int e = eb; e < ee; ++e) local += chunks_of<G>(s, e) * p.n_tiles;
+    int incl = local;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += o;
+    }
+    if (lane == 31) s.warp_tot[warp] = incl;
+    __syncthreads();
+    int run = incl - local;
+    for (int w = 0; w < warp; ++w) run += s.warp_tot[w];
+    for (int e = eb; e < ee; ++e) {
+      s.cum[e] = run;
+      run += chunks_of<G>(s, e) * p.n_tiles;
+    }
+    if (eb < E && ee == E) s.cum[E] = run;
+  }
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&s.full_bar[i], 2);  // the producer's expect_tx and the scale warp
+      mbar_init(&s.empty_bar[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.acc_full_bar[i], 1);
+      mbar_init(&s.acc_empty_bar[i], kEpiWarps);
+    }
+    mbar_init(&s.mma_done_bar, 1);
+    for (int i = 0; i < kUnitQ; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_empty[i], 1 + kEpiWarps + S);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a64)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a16)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_b)) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s.tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem_base = s.tmem_base;
+  const int total = s.cum[E];
+  const int num_kb = (p.steps + kSteps - 1) / kSteps;
+  volatile int32_t* abort = &s.abort;
+
+  // Columns of a unit's tile and whether its second box holds any of them.
+  auto cols_of = [&](const Unit& u) { return min(p.out_tile_cols, p.n_out - u.n * p.out_tile_cols); };
+  auto boxes_of = [&](const Unit& u) { return SWIGLU || cols_of(u) > kBoxRows ? 2 : 1; };
+
+  if (warp == 0) {
+    // ===================== TMA producer =====================
+    if (lane == 0) {
+      // Weights: normal eviction, so the other chunks of an expert find them
+      // in L2; tokens are read by every n-tile and stay.
+      const uint64_t pol_w = policy_evict_normal();
+      const uint64_t pol_a = policy_evict_last();
+      bool ok = true;
+      uint32_t j = 0;  // stages issued so far
+      uint32_t qn = 0;
+      for (int i = 0; ok; ++i, ++qn) {
+        const int qslot = qn % kUnitQ;
+        if (!mbar_wait(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort,
+                       kDevErrGemmProducerWait, true)) {
+          ok = false;
+          break;
+        }
+        int unit = p.counter ? atomicAdd(p.counter, 1) : blockIdx.x + i * static_cast<int>(gridDim.x);
+        if (unit >= total) unit = -1;
+        s.unit_q[qslot] = unit;
+        mbar_arrive(&s.q_full[qslot]);
+        if (unit < 0) break;
+        const Unit u = decode_unit<G>(s, E, unit);
+        const int nn = (u.rows + 15) & ~15;
+        const int boxes = boxes_of(u);
+        const int brow = u.e * p.b_rows + u.n * p.b_tile_rows;
+        const uint8_t* sf = p.b_sf + static_cast<int64_t>(u.e * p.sf_tiles + u.n * p.sf_tile_step) *
+                                         p.steps * kSfTile;
+        for (int kb = 0; kb < num_kb; ++kb, ++j) {
+          const int slot = j % S;
+          if (!mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait,
+                         true)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = s.ring[slot];
+          uint64_t* full = &s.full_bar[slot];
+          const uint32_t sf_bytes = min(kSteps, p.steps - kb * kSteps) * kSfTile;
+          mbar_expect_tx(full, nn * kRowBytes + boxes * (kBoxBytes + sf_bytes));
+          for (int b = 0; b < boxes; ++b) {
+            tma_load_2d(st + b * kBoxBytes, &tmap_b, full, kb * kRowBytes, brow + b * p.b_second,
+                        pol_w);
+            bulk_load(st + kSfBOff + b * kSfBoxBytes,
+                      sf + (static_cast<int64_t>(b * p.sf_second) * p.steps + kb * kSteps) * kSfTile,
+                      sf_bytes, full);
+          }
+          int r = 0;
+          for (; r + 64 <= nn; r += 64)
+            tma_load_2d(st + kTokOff + r * kRowBytes, &tmap_a64, full, kb * kRowBytes, u.row0 + r,
+                        pol_a);
+          for (; r < nn; r += 16)
+            tma_load_2d(st + kTokOff + r * kRowBytes, &tmap_a16, full, kb * kRowBytes, u.row0 + r,
+                        pol_a);
+        }
+      }
+      if (!ok) {  // let every issued load land before the CTA can exit
+        for (uint32_t d = j > S ? j - S : 0; d < j; ++d)
+          mbar_wait(&s.full_bar[d % S], (d / S) & 1u, abort, kDevErrGemmProducerWait, false);
+      }
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer =====================
+    if (lane == 0) {
+      uint32_t ac = 0;  // accumulator slots taken so far
+      uint32_t j = 0;   // stages consumed so far
+      bool ok = true;
+      for (uint32_t qn = 0; ok; ++qn) {
+        const int qslot = qn % kUnitQ;
+        if (!mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmMmaWait, true)) break;
+        const int unit = s.unit_q[qslot];
+        mbar_arrive(&s.q_empty[qslot]);
+        if (unit < 0) break;
+        const Unit u = decode_unit<G>(s, E, unit);
+        const int nn = (u.rows + 15) & ~15;
+        const int boxes = boxes_of(u);
+        const int halves = nn > 128 ? 2 : 1;
+        const uint32_t idesc = fp4_idesc(nn);
+        const bool two = nn > kAccCols / 2;  // the unit takes both slots
+        const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
+        if (!mbar_wait(&s.acc_empty_bar[acc0], ((ac >> 1) & 1u) ^ 1u, abort, kDevErrGemmMmaWait,
+                       true) ||
+            (two && !mbar_wait(&s.acc_empty_bar[acc1], (((ac + 1) >> 1) & 1u) ^ 1u, abort,
+                               kDevErrGemmMmaWait, true))) {
+          ok = false;
+          break;
+        }
+        ac += two ? 2u : 1u;
+        tc_fence_after();
+        const uint32_t d0 = tmem_base + (two ? 0u : acc0 * kAccCols);
+        const uint32_t d1 = d0 + (two ? kAccCols : kAccCols / 2);
+        for (int kb = 0; kb < num_kb; ++kb, ++j) {
+          const int slot = j % S;
+          // The scale buffer was last read by the MMAs of two stages before.
+          if (j >= 2 && !mbar_wait(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u, abort,
+                                   kDevErrGemmMmaWait, true)) {
+            ok = false;
+            break;
+          }
+          if (!mbar_wait(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmMmaWait, true)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(s.ring[slot]);
+          const uint32_t sfb = tmem_base + kSfCol + (j & 1u) * kSfBufCols;  // weights
+          const uint32_t sft = sfb + 2 * kSteps * 4;                        // tokens
+          const int steps = min(kSteps, p.steps - kb * kSteps);
+          for (int k = 0; k < steps; ++k) {
+            for (int b = 0; b < boxes; ++b)
+              tmem_copy_sf(sfb + (k * 2 + b) * 4, st + kSfBOff + b * kSfBoxBytes + k * kSfTile);
+            for (int h = 0; h < halves; ++h)
+              tmem_copy_sf(sft + k * 8 + h * 4, st + kSfAOff + (k * G::kHalves + h) * kSfTile);
+          }
+          for (int k = 0; k < steps; ++k) {
+            const uint64_t tok = smem_desc_sw128(st + kTokOff + k * 32);
+            const uint32_t acc_in = (kb | k) != 0 ? 1u : 0u;
+            umma_fp4(d0, smem_desc_sw128(st + k * 32), tok, idesc, sfb + k * 8, sft + k * 8, acc_in);
+            if (boxes == 2)
+              umma_fp4(d1, smem_desc_sw128(st + kBoxBytes + k * 32), tok, idesc, sfb + k * 8 + 4,
+                       sft + k * 8, acc_in);
+          }
+          umma_commit(&s.empty_bar[slot]);
+        }
+        if (ok) {
+          umma_commit(&s.acc_full_bar[acc0]);
+          if (two) umma_commit(&s.acc_full_bar[acc1]);
+        }
+      }
+      // Outstanding MMAs read shared memory and write TMEM: finish them first.
+      umma_commit(&s.mma_done_bar);
+      mbar_wait(&s.mma_done_bar, 0, abort, kDevErrGemmMmaWait, false);
+    }
+  } else if (warp >= kFirstSfWarp) {
+    // ===================== activation scales (warps 10..) =====================
+    const uint32_t mine = static_cast<uint32_t>(warp - kFirstSfWarp);  // its ring slot
+    const int sf_row = p.steps * 4;  // scale bytes of a row
+    uint32_t j = 0;
+    bool ok = true;
+    for (uint32_t qn = 0; ok; ++qn) {
+      const int qslot = qn % kUnitQ;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort,
+                                             kDevErrGemmScaleWait, true));
+      if (!ok) break;
+      const int unit = s.unit_q[qslot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.q_empty[qslot]);
+      if (unit < 0) break;
+      const Unit u = decode_unit<G>(s, E, unit);
+      const int halves = u.rows > 128 ? 2 : 1;
+      for (int kb = 0; kb < num_kb; ++kb, ++j) {
+        const uint32_t slot = j % S;
+        if (slot != mine) continue;
+        const int steps = min(kSteps, p.steps - kb * kSteps);
+        // Row 32 q + lane of each half: its scales of the stage's four MMAs.
+        // Rows past the unit get zeros; their results are not stored.
+        uint32_t w[G::kHalves][4][kSteps];
+#pragma unroll
+        for (int h = 0; h < G::kHalves; ++h)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = h * 128 + q * 32 + lane;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) w[h][q][k] = 0u;
+            if (r < u.rows) {
+              const uint8_t* src = p.a_sf + static_cast<int64_t>(u.row0 + r) * sf_row + kb * (4 * kSteps);
+              if (p.wide_scales) {
+                const uint4 v = ldg_nc_v4(src);
+                w[h][q][0] = v.x;
+                w[h][q][1] = v.y;
+                w[h][q][2] = v.z;
+                w[h][q][3] = v.w;
+              } else {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+                  if (k < steps) w[h][q][k] = __ldg(reinterpret_cast<const uint32_t*>(src) + k);
+              }
+            }
+          }
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort,
+                                               kDevErrGemmScaleWait, true));
+        if (!ok) break;
+        uint8_t* dst = s.ring[slot] + kSfAOff + lane * 16;
+#pragma unroll
+        for (int h = 0; h < G::kHalves; ++h)
+          if (h < halves)
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+              *reinterpret_cast<uint4*>(dst + (k * G::kHalves + h) * kSfTile) =
+                  make_uint4(w[h][0][k], w[h][1][k], w[h][2][k], w[h][3][k]);
+        // Written by ordinary stores, read by tcgen05.cp through the async proxy.
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.full_bar[slot]);
+      }
+    }
+  } else {
+    // ===================== epilogue (warps 2..9) =====================
+    const int q = warp & 3;           // TMEM lane quarter this warp may access
+    const int grp = (warp - 2) >> 2;  // chunks of 16 tokens this warp drains: grp, grp + 2, ...
+    uint8_t* turn = s.turn[warp - 2];
+    const float ga = p.a_global ? __ldg(p.a_global) : 1.0f;
+    const float go = SWIGLU && p.out_global ? __ldg(p.out_global) : 1.0f;
+    const float six_go = __fmul_rn(6.0f, go);
+    uint32_t ac = 0;
+    for (uint32_t qn = 0;; ++qn) {
+      const int qslot = qn % kUnitQ;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort,
+                                             kDevErrGemmEpilogueWait, true)))
+        break;
+      const int unit = s.unit_q[qslot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.q_empty[qslot]);
+      if (unit < 0) break;
+      const Unit u = decode_unit<G>(s, E, unit);
+      const int nn = (u.rows + 15) & ~15;
+      const bool two = nn > kAccCols / 2;
+      const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
+      bool got = mbar_wait(&s.acc_full_bar[acc0], (ac >> 1) & 1u, abort, kDevErrGemmEpilogueWait, true);
+      if (two)
+        got = mbar_wait(&s.acc_full_bar[acc1], ((ac + 1) >> 1) & 1u, abort, kDevErrGemmEpilogueWait,
+                        true) && got;
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after();
+      const uint32_t d0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                          (two ? 0u : acc0 * kAccCols);
+      const uint32_t d1 = d0 + (two ? kAccCols : kAccCols / 2);
+      const float alpha = p.b_global ? __fmul_rn(ga, __ldg(p.b_global + u.e)) : ga;
+      const int col0 = u.n * p.out_tile_cols;
+      const int cols = cols_of(u);
+      const int boxes = boxes_of(u);
+      const int tok = lane >> 1;                  // after the turn: token and
+      const int feat = q * 32 + (lane & 1) * 16;  // first of 16 output columns of the box
+      const uint4* mine = reinterpret_cast<const uint4*>(turn + tok * kStagePitch + (lane & 1) * 32);
+#pragma unroll 1
+      for (int t0 = grp * 16; t0 < nn; t0 += 32) {
+        uint32_t v0[16], v1[16];
+        tmem_ld16(d0 + t0, v0);
+        if (boxes == 2) tmem_ld16(d1 + t0, v1);
+        tmem_ld_wait();
+        const int64_t row = u.row0 + t0 + tok;
+        const bool live = t0 + tok < u.rows;
+#pragma unroll 1
+        for (int b = 0; b < (SWIGLU ? 1 : boxes); ++b) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            __nv_bfloat16 h;
+            if (SWIGLU) {
+              const float g = round_bf16(__fmul_rn(alpha, __uint_as_float(v0[i])));
+              const float up = round_bf16(__fmul_rn(alpha, __uint_as_float(v1[i])));
+              h = __float2bfloat16_rn(swiglu_f32(g, up, p.swiglu_limit));
+            } else {
+              h = __float2bfloat16_rn(__fmul_rn(alpha, __uint_as_float(b == 0 ? v0[i] : v1[i])));
+            }
+            *reinterpret_cast<__nv_bfloat16*>(turn + i * kStagePitch + lane * 2) = h;
+          }
+          __syncwarp();
+          const uint4 lo = mine[0], hi = mine[1];
+          __syncwarp();
+          const int f = b * kBoxRows + feat;
+          if (live && f < cols) {
+            if (SWIGLU) {
+              const Fp4Block blk = fp4_quantize16<__nv_bfloat16>(lo, hi, go, six_go);
+              const int64_t at = (row * p.n_out + col0 + f) / kFp4Block;
+              reinterpret_cast<uint2*>(p.out_codes)[at] = blk.codes;
+              p.out_sf[at] = static_cast<uint8_t>(blk.scale);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(p.D + row * p.n_out + col0 + f);
+              dst[0] = lo;
+              dst[1] = hi;
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&s.acc_empty_bar[acc0]);
+        if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
+      }
+      ac += two ? 2u : 1u;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(kTmemCols)
+                 : "memory");
+  }
+}
+
+// ---- host side -----------------------------------------------------------------
+
+// 2-D byte map over a [outer, inner] row-major tensor, box [box_rows, 128 bytes],
+// 128-byte swizzle, zero fill out of bounds (code 0 = value 0).
+lsek_status make_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                     uint32_t box_rows) {
+  EncodeTiledFn fn = tensor_map_encoder();
+  if (fn == nullptr) return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {inner, outer};
+  const cuuint64_t strides[1] = {inner};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kRowBytes), box_rows};
+  const cuuint32_t es[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                        strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return LSEK_OK;
+}
+
+template <bool SWIGLU, class G>
+lsek_status launch_geom(Params p, const void* A, const void* B, int K, cudaStream_t st) {
+  static PerDeviceOnce attrs;
+  const cudaError_t ae = once_per_device(attrs, [] {
+    return cudaFuncSetAttribute(fp4_gemm_kernel<SWIGLU, G>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(smem_bytes<G>()));
+  });
+  if (ae != cudaSuccess) return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: %s", cudaGetErrorString(ae));
+  CUtensorMap a64, a16, b;
+  const uint64_t row_bytes = static_cast<uint64_t>(K) / 2;
+  lsek_status s = make_map(&a64, A, row_bytes, static_cast<uint64_t>(p.rows), 64u);
+  if (s == LSEK_OK) s = make_map(&a16, A, row_bytes, static_cast<uint64_t>(p.rows), 16u);
+  if (s == LSEK_OK)
+    s = make_map(&b, B, row_bytes, static_cast<uint64_t>(p.num_experts) * p.b_rows,
+                 static_cast<uint32_t>(kBoxRows));
+  if (s != LSEK_OK) return s;
+  if (p.counter != nullptr) LSEK_CUDA_TRY(cudaMemsetAsync(p.counter, 0, sizeof(int32_t), st));
+  // At most rows / kTok full chunks and one partial chunk per non-empty expert.
+  const int64_t experts = p.num_experts < p.rows ? p.num_experts : p.rows;
+  const int64_t max_units = (p.rows / G::kTok + experts) * static_cast<int64_t>(p.n_tiles);
+  const int grid = static_cast<int>(max_units < num_sms() ? max_units : num_sms());
+  fp4_gemm_kernel<SWIGLU, G><<<grid, G::kThreads, smem_bytes<G>(), st>>>(a64, a16, b, p);
+  return check_launch(SWIGLU ? "grouped_gemm_swiglu_nvfp4" : "grouped_gemm_nvfp4");
+}
+
+}  // namespace fp4
+
+lsek_status fp4_take_device_error(int32_t* code) {
+  int32_t zero = 0;
+  LSEK_CUDA_TRY(cudaMemcpyFromSymbol(code, g_device_error, sizeof(int32_t)));
+  LSEK_CUDA_TRY(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int32_t)));
+  return LSEK_OK;
+}
+
+// Both products; D for the plain one, h_codes / h_scales for gate/up + SwiGLU
+// (n_out = I there).  max_rows_per_expert: an upper bound, or -1; every
+// argument has been checked.
+lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales, const void* A,
+                             const void* a_scales, const void* B, const void* b_tiles,
+                             const int32_t* offsets, const float* a_global, const float* b_global,
+                             const float* out_global, int E, int rows, int n_out, int K,
+                             float limit, int32_t* counter, cudaStream_t st,
+                             int max_rows_per_expert) {
+  using namespace fp4;
+  if (rows == 0 || n_out == 0) return LSEK_OK;
+  Params p{};
+  p.offsets = offsets;
+  p.num_experts = E;
+  p.rows = rows;
+  p.steps = K / kStepK;
+  p.a_sf = static_cast<const uint8_t*>(a_scales);
+  p.b_sf = static_cast<const uint8_t*>(b_tiles);
+  p.a_global = a_global;
+  p.b_global = b_global;
+  p.out_global = out_global;
+  p.D = static_cast<__nv_bfloat16*>(D);
+  p.out_codes = static_cast<uint8_t*>(h_codes);
+  p.out_sf = static_cast<uint8_t*>(h_scales);
+  p.n_out = n_out;
+  p.swiglu_limit = limit;
+  p.counter = counter;
+  p.wide_scales = K % (kSteps * kStepK) == 0;
+  const int col_tiles = static_cast<int>(ceil_div(n_out, kBoxRows));
+  if (swiglu) {  // gate rows and up rows are tiled apart
+    p.b_rows = 2 * n_out;
+    p.b_tile_rows = kBoxRows;
+    p.b_second = n_out;
+    p.sf_tiles = 2 * col_tiles;
+    p.sf_tile_step = 1;
+    p.sf_second = col_tiles;
+    p.out_tile_cols = kBoxRows;
+  } else {
+    p.b_rows = n_out;
+    p.b_tile_rows = 2 * kBoxRows;
+    p.b_second = kBoxRows;
+    p.sf_tiles = col_tiles;
+    p.sf_tile_step = 2;
+    p.sf_second = 1;
+    p.out_tile_cols = 2 * kBoxRows;
+  }
+  p.n_tiles = static_cast<int>(ceil_div(n_out, p.out_tile_cols));
+  const int bound = max_rows_per_expert >= 0 && max_rows_per_expert < rows ? max_rows_per_expert : rows;
+  if (bound <= GeomDecode::kTok && E <= GeomDecode::kMaxE)
+    return swiglu ? launch_geom<true, GeomDecode>(p, A, B, K, st)
+                  : launch_geom<false, GeomDecode>(p, A, B, K, st);
+  return swiglu ? launch_geom<true, GeomFull>(p, A, B, K, st)
+                : launch_geom<false, GeomFull>(p, A, B, K, st);
+}
+
+namespace {
+
+lsek_status check_fp4_gemm(const char* name, int E, int rows, int n_out, int n_weights, int K,
+                           std::initializer_list<const void*> sixteen, const int32_t* offsets,
+                           const void* workspace) {
+  LSEK_REQUIRE(E >= 1, "%s: num_experts must be >= 1", name);
+  LSEK_REQUIRE(rows >= 0 && n_out >= 0 && K >= 0, "%s: sizes must be >= 0", name);
+  if (E > fp4::kMaxExperts)
+    return fail(LSEK_ERR_UNSUPPORTED, "%s: num_experts must be <= %d", name, fp4::kMaxExperts);
+  LSEK_REQUIRE(K % fp4::kStepK == 0, "%s: K must be a multiple of %d, got %d", name, fp4::kStepK, K);
+  LSEK_REQUIRE(n_out % 32 == 0, "%s: output width must be a multiple of 32, got %d", name, n_out);
+  LSEK_REQUIRE(static_cast<int64_t>(E) * n_weights < (1ll << 31),
+               "%s: num_experts * weight rows must fit in int32", name);
+  if (rows == 0 || n_out == 0) return LSEK_OK;
+  LSEK_REQUIRE(K > 0, "%s: K must be > 0 when there are rows to compute", name);
+  LSEK_REQUIRE(offsets != nullptr, "%s: expert_offsets is NULL", name);
+  for (const void* t : sixteen) {
+    LSEK_REQUIRE(t != nullptr, "%s: NULL tensor pointer", name);
+    LSEK_REQUIRE(reinterpret_cast<uintptr_t>(t) % 16 == 0, "%s: tensors must be 16-byte aligned", name);
+  }
+  LSEK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "%s: workspace must be 4-byte aligned", name);
+  return LSEK_OK;
+}
+
+int32_t* counter_in(void* workspace, size_t workspace_bytes) {
+  return workspace != nullptr && workspace_bytes >= sizeof(int32_t) ? static_cast<int32_t*>(workspace)
+                                                                    : nullptr;
+}
+
+}  // namespace
+}  // namespace lsek
+
+extern "C" lsek_status lsek_grouped_gemm_nvfp4(void* D, const void* A, const void* a_scales,
+                                               const void* B, const void* b_scale_tiles,
+                                               const int32_t* expert_offsets,
+                                               const float* a_global_scale,
+                                               const float* b_global_scale, int32_t num_experts,
+                                               int32_t rows, int32_t N, int32_t K, void* workspace,
+                                               size_t workspace_bytes, void* stream) {
+  using namespace lsek;
+  const lsek_status s = check_fp4_gemm("grouped_gemm_nvfp4", num_experts, rows, N, N, K,
+                                       {D, A, a_scales, B, b_scale_tiles}, expert_offsets, workspace);
+  if (s != LSEK_OK) return s;
+  return grouped_gemm_fp4(false, D, nullptr, nullptr, A, a_scales, B, b_scale_tiles, expert_offsets,
+                          a_global_scale, b_global_scale, nullptr, num_experts, rows, N, K, 0.0f,
+                          counter_in(workspace, workspace_bytes), static_cast<cudaStream_t>(stream), -1);
+}
+
+extern "C" lsek_status lsek_grouped_gemm_swiglu_nvfp4(
+    void* h_codes, void* h_scales, const void* A, const void* a_scales, const void* W_gu,
+    const void* gu_scale_tiles, const int32_t* expert_offsets, const float* a_global_scale,
+    const float* gu_global_scale, const float* h_global_scale, int32_t num_experts, int32_t rows,
+    int32_t I, int32_t K, float swiglu_limit, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  using namespace lsek;
+  LSEK_REQUIRE(I >= 0 && I < (1 << 30), "grouped_gemm_swiglu_nvfp4: I out of range");
+  const lsek_status s =
+      check_fp4_gemm("grouped_gemm_swiglu_nvfp4", num_experts, rows, I, 2 * I, K,
+                     {h_codes, h_scales, A, a_scales, W_gu, gu_scale_tiles}, expert_offsets, workspace);
+  if (s != LSEK_OK) return s;
+  LSEK_REQUIRE(swiglu_limit >= 0.0f, "grouped_gemm_swiglu_nvfp4: swiglu_limit must be >= 0");
+  return grouped_gemm_fp4(true, nullptr, h_codes, h_scales, A, a_scales, W_gu, gu_scale_tiles,
+                          expert_offsets, a_global_scale, gu_global_scale, h_global_scale,
+                          num_experts, rows, I, K, swiglu_limit, counter_in(workspace, workspace_bytes),
+                          static_cast<cudaStream_t>(stream), -1);
+}

@@ -406,6 +406,275 @@ void moe_layer_forward_out(torch::Tensor out, torch::Tensor hidden, torch::Tenso
       stream_of(hidden)));
 }
 
+// ---- NVFP4 experts -------------------------------------------------------------
+
+// One float32 on the device for each of n groups; absent means 1.
+const float* global_ptr(const char* op, const char* what, const c10::optional<torch::Tensor>& g,
+                        int64_t n, const torch::Tensor& like) {
+  if (!g.has_value()) return nullptr;
+  TORCH_CHECK(g->is_cuda() && g->device() == like.device(), op, ": ", what,
+              " must be on the same CUDA device as the data");
+  TORCH_CHECK(g->is_contiguous() && g->scalar_type() == at::kFloat && g->numel() == n, op, ": ",
+              what, " must be a contiguous float32 tensor of ", n, " value(s)");
+  return g->data_ptr<float>();
+}
+
+// groups x rows x K of a 2-D (one group) or 3-D tensor.
+struct RowsOf {
+  int64_t groups, rows, k;
+};
+RowsOf rows_of(const char* op, const torch::Tensor& t) {
+  TORCH_CHECK(t.dim() == 2 || t.dim() == 3, op, ": a 2-D [rows, K] or 3-D [groups, rows, K] tensor expected");
+  const bool g = t.dim() == 3;
+  return {g ? t.size(0) : 1, t.size(g ? 1 : 0), t.size(g ? 2 : 1)};
+}
+
+void check_codes(const char* op, const char* what, const torch::Tensor& codes,
+                 const torch::Tensor& scales) {
+  TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), op, ": ", what, " and its scales must be on CUDA");
+  TORCH_CHECK(codes.device() == scales.device(), op, ": ", what, " and its scales must be on one device");
+  TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous(), op, ": ", what,
+              " and its scales must be contiguous");
+  TORCH_CHECK(codes.scalar_type() == at::kByte, op, ": ", what, " must be uint8 (two codes a byte)");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat8_e4m3fn, op, ": the scales of ", what,
+              " must be float8_e4m3fn");
+}
+
+// Rows of codes with rows of scales: sizes agree but for the factor 8.
+void check_row_scales(const char* op, const char* what, const torch::Tensor& codes,
+                      const torch::Tensor& scales) {
+  check_codes(op, what, codes, scales);
+  TORCH_CHECK(codes.dim() == scales.dim(), op, ": ", what, " and its scales must have the same rank");
+  for (int64_t d = 0; d + 1 < codes.dim(); ++d)
+    TORCH_CHECK(codes.size(d) == scales.size(d), op, ": ", what, " and its scales disagree on the rows");
+  TORCH_CHECK(codes.size(-1) == 8 * scales.size(-1), op, ": ", what,
+              " must hold 8 bytes of codes for each scale");
+}
+
+std::vector<torch::Tensor> nvfp4_quantize(torch::Tensor x, c10::optional<torch::Tensor> global_scale) {
+  const char* op = "nvfp4_quantize";
+  TORCH_CHECK(x.is_cuda(), op, ": x must be on CUDA");
+  TORCH_CHECK(x.is_contiguous(), op, ": x must be contiguous");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, op,
+              ": x must be bfloat16 or float16");
+  const RowsOf r = rows_of(op, x);
+  TORCH_CHECK(r.k % 16 == 0, op, ": the row length must be a multiple of 16, got ", r.k);
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  const float* g = global_ptr(op, "global_scale", global_scale, r.groups, x);
+  auto shape = x.sizes().vec();
+  shape.back() = r.k / 2;
+  auto codes = torch::empty(shape, x.options().dtype(at::kByte));
+  shape.back() = r.k / 16;
+  auto scales = torch::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  check_status(lsek_nvfp4_quantize(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), g, r.groups,
+                                   r.rows, to_i32(r.k, "K"), dtype_code(x), stream_of(x)));
+  return {codes, scales};
+}
+
+torch::Tensor nvfp4_dequantize(torch::Tensor codes, torch::Tensor scales,
+                               c10::optional<torch::Tensor> global_scale,
+                               c10::optional<at::ScalarType> dtype_opt) {
+  const char* op = "nvfp4_dequantize";
+  check_row_scales(op, "codes", codes, scales);
+  const at::ScalarType dtype = dtype_opt.value_or(at::kBFloat16);
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat, op,
+              ": dtype must be bfloat16, float16 or float32");
+  const RowsOf r = rows_of(op, codes);
+  const c10::cuda::OptionalCUDAGuard guard(codes.device());
+  const float* g = global_ptr(op, "global_scale", global_scale, r.groups, codes);
+  auto shape = codes.sizes().vec();
+  shape.back() = 2 * r.k;
+  auto out = torch::empty(shape, codes.options().dtype(dtype));
+  check_status(lsek_nvfp4_dequantize(out.data_ptr(), codes.data_ptr(), scales.data_ptr(), g, r.groups,
+                                     r.rows, to_i32(2 * r.k, "K"), dtype_code(out),
+                                     stream_of(codes)));
+  return out;
+}
+
+std::vector<torch::Tensor> moe_permute_nvfp4(torch::Tensor hidden_states, torch::Tensor topk_indices,
+                                             int64_t num_experts,
+                                             c10::optional<torch::Tensor> global_scale) {
+  const char* op = "moe_permute_nvfp4";
+  TORCH_CHECK(hidden_states.is_cuda(), op, ": hidden_states must be on CUDA");
+  TORCH_CHECK(topk_indices.is_cuda() && topk_indices.device() == hidden_states.device(), op,
+              ": topk_indices must be on CUDA, on the device of hidden_states");
+  TORCH_CHECK(hidden_states.is_contiguous() && topk_indices.is_contiguous(), op,
+              ": tensors must be contiguous");
+  TORCH_CHECK(hidden_states.scalar_type() == at::kBFloat16, op, ": hidden_states must be bfloat16");
+  TORCH_CHECK(hidden_states.dim() == 2, op, ": hidden_states must be 2D");
+  TORCH_CHECK(topk_indices.dim() == 2, op, ": topk_indices must be 2D [num_tokens, topk]");
+  TORCH_CHECK(topk_indices.scalar_type() == at::kInt, op, ": topk_indices must be int32");
+  TORCH_CHECK(topk_indices.size(0) == hidden_states.size(0), op,
+              ": topk_indices and hidden_states disagree on num_tokens");
+  const int64_t T = hidden_states.size(0), H = hidden_states.size(1), k = topk_indices.size(1);
+  TORCH_CHECK(H % 16 == 0, op, ": hidden_dim must be a multiple of 16, got ", H);
+  TORCH_CHECK(num_experts >= 1 && num_experts <= 1023, op, ": num_experts must be in [1, 1023]");
+  const c10::cuda::OptionalCUDAGuard guard(hidden_states.device());
+  const float* g = global_ptr(op, "global_scale", global_scale, 1, hidden_states);
+  const int64_t n = T * k;
+  auto codes = torch::empty({n, H / 2}, hidden_states.options().dtype(at::kByte));
+  auto scales = torch::empty({n, H / 16}, hidden_states.options().dtype(at::kFloat8_e4m3fn));
+  auto offsets = torch::empty({num_experts + 1}, topk_indices.options());
+  auto s2d = torch::empty({n}, topk_indices.options());
+  auto perm = torch::empty({n}, topk_indices.options());
+  check_status(lsek_moe_permute_nvfp4(
+      codes.data_ptr(), scales.data_ptr(), offsets.data_ptr<int32_t>(), s2d.data_ptr<int32_t>(),
+      perm.data_ptr<int32_t>(), hidden_states.data_ptr(), topk_indices.data_ptr<int32_t>(), g,
+      to_i32(T, "num_tokens"), to_i32(k, "topk"), to_i32(H, "hidden_dim"),
+      static_cast<int32_t>(num_experts), stream_of(hidden_states)));
+  return {codes, scales, offsets, s2d, perm};
+}
+
+// Weights [E, parts * R, K/2] with tiled scales [E, parts * ceil(R / 128), K / 64, 512].
+void check_fp4_weights(const char* op, const char* what, const torch::Tensor& W,
+                       const torch::Tensor& tiles, int64_t K, int64_t parts) {
+  check_codes(op, what, W, tiles);
+  TORCH_CHECK(W.dim() == 3, op, ": ", what, " must be [E, rows, K/2]");
+  TORCH_CHECK(W.size(2) * 2 == K, op, ": ", what, " and the activations disagree on K");
+  TORCH_CHECK(K % 64 == 0, op, ": K must be a multiple of 64, got ", K);
+  TORCH_CHECK(W.size(1) % parts == 0, op, ": ", what, " must hold ", parts, " equal parts of rows");
+  const int64_t tall = parts * ((W.size(1) / parts + 127) / 128);
+  TORCH_CHECK(tiles.dim() == 4 && tiles.size(0) == W.size(0) && tiles.size(1) == tall &&
+                  tiles.size(2) == K / 64 && tiles.size(3) == 512,
+              op, ": the scales of ", what, " must be tiled, [", W.size(0), ", ", tall, ", ", K / 64,
+              ", 512] (nvfp4_tile_scales, parts=", parts, ")");
+}
+
+void check_fp4_rows(const char* op, const torch::Tensor& A, const torch::Tensor& A_scales,
+                    const torch::Tensor& W, const torch::Tensor& offsets) {
+  check_row_scales(op, "A", A, A_scales);
+  TORCH_CHECK(A.dim() == 2, op, ": A must be [rows, K/2]");
+  TORCH_CHECK(offsets.is_cuda() && offsets.is_contiguous() && offsets.scalar_type() == at::kInt, op,
+              ": expert_offsets must be a contiguous int32 CUDA tensor");
+  TORCH_CHECK(A.device() == W.device() && A.device() == offsets.device(), op,
+              ": tensors must be on one device");
+  TORCH_CHECK(offsets.numel() == W.size(0) + 1, op, ": expert_offsets must hold E+1 entries");
+}
+
+torch::Tensor grouped_gemm_nvfp4(torch::Tensor A, torch::Tensor A_scales, torch::Tensor B,
+                                 torch::Tensor B_scales, torch::Tensor expert_offsets,
+                                 c10::optional<torch::Tensor> a_global_scale,
+                                 c10::optional<torch::Tensor> b_global_scale) {
+  const char* op = "grouped_gemm_nvfp4";
+  check_fp4_rows(op, A, A_scales, B, expert_offsets);
+  const int64_t K = 2 * A.size(1);
+  check_fp4_weights(op, "B", B, B_scales, K, 1);
+  const c10::cuda::OptionalCUDAGuard guard(A.device());
+  const float* ga = global_ptr(op, "a_global_scale", a_global_scale, 1, A);
+  const float* gb = global_ptr(op, "b_global_scale", b_global_scale, B.size(0), A);
+  auto D = torch::empty({A.size(0), B.size(1)}, A.options().dtype(at::kBFloat16));
+  auto ws = torch::empty({LSEK_GEMM_WORKSPACE_BYTES}, A.options());
+  check_status(lsek_grouped_gemm_nvfp4(
+      D.data_ptr(), A.data_ptr(), A_scales.data_ptr(), B.data_ptr(), B_scales.data_ptr(),
+      expert_offsets.data_ptr<int32_t>(), ga, gb, to_i32(B.size(0), "E"), to_i32(A.size(0), "rows"),
+      to_i32(B.size(1), "N"), to_i32(K, "K"), ws.data_ptr(), LSEK_GEMM_WORKSPACE_BYTES, stream_of(A)));
+  return D;
+}
+
+std::vector<torch::Tensor> grouped_gemm_swiglu_nvfp4(
+    torch::Tensor A, torch::Tensor A_scales, torch::Tensor W_gu, torch::Tensor W_gu_scales,
+    torch::Tensor expert_offsets, c10::optional<torch::Tensor> a_global_scale,
+    c10::optional<torch::Tensor> w_global_scale, c10::optional<torch::Tensor> out_global_scale,
+    double swiglu_limit) {
+  const char* op = "grouped_gemm_swiglu_nvfp4";
+  check_fp4_rows(op, A, A_scales, W_gu, expert_offsets);
+  const int64_t K = 2 * A.size(1);
+  check_fp4_weights(op, "W_gu", W_gu, W_gu_scales, K, 2);
+  const c10::cuda::OptionalCUDAGuard guard(A.device());
+  const float* ga = global_ptr(op, "a_global_scale", a_global_scale, 1, A);
+  const float* gw = global_ptr(op, "w_global_scale", w_global_scale, W_gu.size(0), A);
+  const float* go = global_ptr(op, "out_global_scale", out_global_scale, 1, A);
+  const int64_t I = W_gu.size(1) / 2;
+  TORCH_CHECK(I % 32 == 0, op, ": I must be a multiple of 32, got ", I);
+  auto codes = torch::empty({A.size(0), I / 2}, A.options());
+  auto scales = torch::empty({A.size(0), I / 16}, A_scales.options());
+  auto ws = torch::empty({LSEK_GEMM_WORKSPACE_BYTES}, A.options());
+  check_status(lsek_grouped_gemm_swiglu_nvfp4(
+      codes.data_ptr(), scales.data_ptr(), A.data_ptr(), A_scales.data_ptr(), W_gu.data_ptr(),
+      W_gu_scales.data_ptr(), expert_offsets.data_ptr<int32_t>(), ga, gw, go,
+      to_i32(W_gu.size(0), "E"), to_i32(A.size(0), "rows"), to_i32(I, "I"), to_i32(K, "K"),
+      static_cast<float>(swiglu_limit), ws.data_ptr(), LSEK_GEMM_WORKSPACE_BYTES, stream_of(A)));
+  return {codes, scales};
+}
+
+int64_t moe_layer_nvfp4_workspace_size(int64_t num_tokens, int64_t hidden_dim, int64_t inter_dim,
+                                       int64_t num_experts, int64_t topk) {
+  return static_cast<int64_t>(lsek_moe_layer_nvfp4_workspace_size(
+      to_i32(num_tokens, "num_tokens"), to_i32(hidden_dim, "hidden_dim"),
+      to_i32(inter_dim, "inter_dim"), to_i32(num_experts, "num_experts"), to_i32(topk, "topk")));
+}
+
+// moe_layer_forward_out on NVFP4 experts (tiled weight scales).
+void moe_layer_forward_nvfp4_out(
+    torch::Tensor out, torch::Tensor hidden, torch::Tensor logits, c10::optional<torch::Tensor> bias,
+    torch::Tensor w_gu, torch::Tensor w_gu_scales, c10::optional<torch::Tensor> w_gu_global_scale,
+    torch::Tensor w_down, torch::Tensor w_down_scales,
+    c10::optional<torch::Tensor> w_down_global_scale,
+    c10::optional<torch::Tensor> hidden_global_scale,
+    c10::optional<torch::Tensor> inter_global_scale, int64_t topk, int64_t n_group,
+    int64_t topk_group, double routed_scaling_factor, bool renormalize, std::string scoring_func,
+    double swiglu_limit, torch::Tensor workspace, c10::optional<torch::Tensor> topk_weights,
+    c10::optional<torch::Tensor> topk_indices, std::vector<int64_t> stage_events) {
+  const char* op = "moe_layer_forward_nvfp4";
+  for (const torch::Tensor* t : {&hidden, &logits, &w_gu, &w_gu_scales, &w_down, &w_down_scales, &out, &workspace}) {
+    TORCH_CHECK(t->is_cuda(), op, ": tensors must be on CUDA");
+    TORCH_CHECK(t->device() == hidden.device(), op, ": tensors must be on one device");
+    TORCH_CHECK(t->is_contiguous(), op, ": tensors must be contiguous");
+  }
+  TORCH_CHECK(hidden.scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16, op,
+              ": hidden and out must be bfloat16");
+  TORCH_CHECK(logits.scalar_type() == at::kFloat, op, ": logits must be float32");
+  TORCH_CHECK(hidden.dim() == 2 && logits.dim() == 2, op, ": hidden [T,H] and logits [T,E] expected");
+  const int64_t T = hidden.size(0), H = hidden.size(1), E = logits.size(1);
+  check_fp4_weights(op, "w_gu", w_gu, w_gu_scales, H, 2);
+  TORCH_CHECK(w_down.dim() == 3, op, ": w_down must be [E, H, I/2]");
+  const int64_t I = 2 * w_down.size(2);
+  check_fp4_weights(op, "w_down", w_down, w_down_scales, I, 1);
+  TORCH_CHECK(logits.size(0) == T && w_gu.size(0) == E && w_down.size(0) == E &&
+                  w_gu.size(1) == 2 * I && w_down.size(1) == H,
+              op, ": inconsistent shapes");
+  TORCH_CHECK(out.dim() == 2 && out.size(0) == T && out.size(1) == H, op, ": out must be [T, H]");
+  TORCH_CHECK(workspace.scalar_type() == at::kByte, op, ": workspace must be uint8");
+  TORCH_CHECK(!bias.has_value() || bias->device() == hidden.device(), op, ": tensors must be on one device");
+  float* wp = nullptr;
+  int32_t* ip = nullptr;
+  if (topk_weights.has_value()) {
+    TORCH_CHECK(topk_weights->scalar_type() == at::kFloat && topk_weights->numel() == T * topk &&
+                    topk_weights->is_contiguous() && topk_weights->device() == hidden.device(),
+                op, ": topk_weights must be a contiguous float32 CUDA tensor of T*topk");
+    wp = topk_weights->data_ptr<float>();
+  }
+  if (topk_indices.has_value()) {
+    TORCH_CHECK(topk_indices->scalar_type() == at::kInt && topk_indices->numel() == T * topk &&
+                    topk_indices->is_contiguous() && topk_indices->device() == hidden.device(),
+                op, ": topk_indices must be a contiguous int32 CUDA tensor of T*topk");
+    ip = topk_indices->data_ptr<int32_t>();
+  }
+  const c10::cuda::OptionalCUDAGuard guard(hidden.device());
+  lsek_topk_gating_params p;
+  p.num_tokens = to_i32(T, "num_tokens");
+  p.num_experts = to_i32(E, "num_experts");
+  p.topk = to_i32(topk, "topk");
+  p.n_group = to_i32(n_group, "n_group");
+  p.topk_group = to_i32(topk_group, "topk_group");
+  p.routed_scaling_factor = static_cast<float>(routed_scaling_factor);
+  p.renormalize = renormalize ? 1 : 0;
+  p.scoring_func = scoring_code(scoring_func);
+  TORCH_CHECK(stage_events.empty() || stage_events.size() == LSEK_LAYER_STAGES + 1, op,
+              ": stage_events must be empty or hold ", LSEK_LAYER_STAGES + 1, " event handles");
+  std::vector<void*> ev(stage_events.size());
+  for (size_t i = 0; i < ev.size(); ++i) ev[i] = reinterpret_cast<void*>(stage_events[i]);
+  check_status(lsek_moe_layer_forward_nvfp4(
+      out.data_ptr(), hidden.data_ptr(), logits.data_ptr<float>(), bias_ptr(bias, E),
+      w_gu.data_ptr(), w_gu_scales.data_ptr(), global_ptr(op, "w_gu_global_scale", w_gu_global_scale, E, hidden),
+      w_down.data_ptr(), w_down_scales.data_ptr(),
+      global_ptr(op, "w_down_global_scale", w_down_global_scale, E, hidden),
+      global_ptr(op, "hidden_global_scale", hidden_global_scale, 1, hidden),
+      global_ptr(op, "inter_global_scale", inter_global_scale, 1, hidden), &p, to_i32(H, "hidden_dim"),
+      to_i32(I, "inter_dim"), static_cast<float>(swiglu_limit), wp, ip, workspace.data_ptr(),
+      static_cast<size_t>(workspace.numel()), ev.empty() ? nullptr : ev.data(), stream_of(hidden)));
+}
+
 // ---- expert-parallel device steps (the exchanges are issued from Python) --------
 
 void check_i32_cuda(const torch::Tensor& t, const char* what) {
@@ -856,6 +1125,35 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("n_group"), py::arg("topk_group"), py::arg("routed_scaling_factor"),
         py::arg("renormalize"), py::arg("scoring_func"), py::arg("swiglu_limit"),
         py::arg("workspace"), py::arg("topk_weights") = py::none(),
+        py::arg("topk_indices") = py::none(), py::arg("stage_events") = std::vector<int64_t>{});
+  m.def("nvfp4_quantize", &nvfp4_quantize, py::arg("x"), py::arg("global_scale") = py::none(),
+        "NVFP4 quantisation of [rows, K] or [groups, rows, K]: [codes uint8 [.., K/2], scales "
+        "float8_e4m3fn [.., K/16]]; global_scale float32, one for each group.");
+  m.def("nvfp4_dequantize", &nvfp4_dequantize, py::arg("codes"), py::arg("scales"),
+        py::arg("global_scale") = py::none(), py::arg("dtype") = py::none(),
+        "code * scale * global_scale in dtype (default bfloat16).");
+  m.def("moe_permute_nvfp4", &moe_permute_nvfp4, py::arg("hidden_states"), py::arg("topk_indices"),
+        py::arg("num_experts"), py::arg("global_scale") = py::none(),
+        "moe_permute with the rows quantised to NVFP4: [codes, scales, offsets, s2d_map, perm_idx].");
+  m.def("grouped_gemm_nvfp4", &grouped_gemm_nvfp4, py::arg("A"), py::arg("A_scales"), py::arg("B"),
+        py::arg("B_scales"), py::arg("expert_offsets"), py::arg("a_global_scale") = py::none(),
+        py::arg("b_global_scale") = py::none(),
+        "grouped_gemm_bf16 on NVFP4 operands: A [rows, K/2] with row scales, B [E, N, K/2] with "
+        "tiled scales -> bf16 [rows, N].");
+  m.def("grouped_gemm_swiglu_nvfp4", &grouped_gemm_swiglu_nvfp4, py::arg("A"), py::arg("A_scales"),
+        py::arg("W_gu"), py::arg("W_gu_scales"), py::arg("expert_offsets"),
+        py::arg("a_global_scale") = py::none(), py::arg("w_global_scale") = py::none(),
+        py::arg("out_global_scale") = py::none(), py::arg("swiglu_limit") = 0.0,
+        "Gate/up product, SwiGLU and NVFP4 quantisation: [codes [rows, I/2], scales [rows, I/16]].");
+  m.def("moe_layer_nvfp4_workspace_size", &moe_layer_nvfp4_workspace_size, py::arg("num_tokens"),
+        py::arg("hidden_dim"), py::arg("inter_dim"), py::arg("num_experts"), py::arg("topk"));
+  m.def("moe_layer_forward_nvfp4_out", &moe_layer_forward_nvfp4_out, py::arg("out"),
+        py::arg("hidden"), py::arg("logits"), py::arg("bias"), py::arg("w_gu"),
+        py::arg("w_gu_scales"), py::arg("w_gu_global_scale"), py::arg("w_down"),
+        py::arg("w_down_scales"), py::arg("w_down_global_scale"), py::arg("hidden_global_scale"),
+        py::arg("inter_global_scale"), py::arg("topk"), py::arg("n_group"), py::arg("topk_group"),
+        py::arg("routed_scaling_factor"), py::arg("renormalize"), py::arg("scoring_func"),
+        py::arg("swiglu_limit"), py::arg("workspace"), py::arg("topk_weights") = py::none(),
         py::arg("topk_indices") = py::none(), py::arg("stage_events") = std::vector<int64_t>{});
   m.def("ep_plan", &ep_plan, py::arg("topk_indices"), py::arg("num_experts"),
         py::arg("world_size"));

@@ -131,3 +131,48 @@ def e4m3_encode(x: np.ndarray, saturate: bool = True) -> np.ndarray:
 def e4m3_round(x: np.ndarray, saturate: bool = True) -> np.ndarray:
     """float32 -> the float32 value of its E4M3 code (e4m3_encode, decoded)."""
     return e4m3_decode(e4m3_encode(x, saturate))
+
+
+# ---------------------------------------------------------------------------
+# NVFP4 quantiser: the definition's float32 steps (numpy rounds each to float32)
+# ---------------------------------------------------------------------------
+
+_E2M1_MAGNITUDES = E2M1_VALUES[:8].astype(np.float64)
+
+
+def e2m1_encode(y: np.ndarray) -> np.ndarray:
+    """float32 -> uint8 E2M1 code: nearest, halves to the even code, magnitudes
+    past 6 saturate; the sign bit is kept."""
+    v = np.asarray(y, dtype=np.float64)
+    a = np.minimum(np.abs(v), 6.0)
+    lo = np.clip(np.searchsorted(_E2M1_MAGNITUDES, a, side="right") - 1, 0, 7)
+    hi = np.minimum(lo + 1, 7)
+    dlo, dhi = a - _E2M1_MAGNITUDES[lo], _E2M1_MAGNITUDES[hi] - a
+    code = np.where((dhi < dlo) | ((dhi == dlo) & (hi % 2 == 0)), hi, lo)
+    return (code + 8 * np.signbit(v)).astype(np.uint8)
+
+
+def nvfp4_quantize(x: np.ndarray, g: float):
+    """x [M, K] (16-bit values as float32), global scale g -> (packed [M, K/2],
+    scales [M, K/16] as E4M3 codes).  scale = e4m3(amax / (6 g)), code =
+    e2m1(x * (1 / (scale * g))), every operation in float32; a block with an
+    infinity or a NaN has scale NaN (0x7F) and codes 0."""
+    v = np.asarray(x, dtype=F32)
+    g = F32(g)
+    b = v.reshape(v.shape[0], -1, 16)
+    with np.errstate(all="ignore"):
+        amax = np.abs(b).max(axis=2)
+        bad = ~np.isfinite(amax)
+        codes8 = e4m3_encode(np.where(bad, F32(0), amax) / (F32(6) * g))
+        s = e4m3_decode(codes8)
+        inv = np.where(s > 0, F32(1) / (s * g), F32(0)).astype(F32)
+        q = e2m1_encode(np.where(bad[..., None], F32(0), b) * inv[..., None])
+    q[bad] = 0
+    codes8[bad] = 0x7F
+    q = q.reshape(v.shape)
+    return (q[:, 0::2] | (q[:, 1::2] << 4)).astype(np.uint8), codes8
+
+
+def nvfp4_values(packed: np.ndarray, scale_codes: np.ndarray) -> np.ndarray:
+    """float64 code * scale of packed codes and E4M3 scale codes."""
+    return nvfp4_dequant(packed, e4m3_decode(scale_codes)).astype(np.float64)
