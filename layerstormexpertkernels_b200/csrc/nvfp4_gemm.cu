@@ -25,30 +25,37 @@
 // K runs in stages of 256 elements: one 128-byte swizzled row of codes, four
 // MMAs of K=64, and 16 scale bytes a row.  The MMA reads scales from TMEM,
 // where a 128-row tile of the four scales of one MMA is 32 lanes x 4 columns
-// (row r in lane r % 32, column r / 32), copied there by tcgen05.cp from a
-// 512-byte image in shared memory.  The weight scales lie in global memory in
-// that order already (they are laid out once) and arrive by bulk copies; the
-// activation scales are plain rows [rows, K/16], which start at any expert
-// boundary, and are turned into the image by the scale warps.
+// (row r in lane r % 32, column r / 32), the same in all four lane quarters.
+// Four scale warps, one for each quarter, write them there with tcgen05.st: a
+// lane takes its 16 bytes of each weight tile from shared memory (the weight
+// scales lie in global memory in that order, laid out once, and arrive by bulk
+// copies) and the 16 bytes of each of its token rows, plain rows [rows, K/16]
+// that start at any expert boundary, from there too where TMA can load them
+// (K % 256 == 0: rows of whole 16-byte pieces) and from global memory
+// otherwise.  (Loading them from global memory always costs 45 to 70 % more
+// time at 128 to 1024 rows an expert: 32 lines a load, in four warps.)  Copying the same tiles
+// with tcgen05.cp takes the tensor pipe about 165 cycles for each 512 bytes, 12
+// to 16 of them a stage, in line with the MMAs: 1.5 times the whole kernel's
+// time (64 experts, H=7168, I=2048: 270 against 183 us at one row an expert).
 //
-// One CTA = 10 warps and one more for each stage:
+// One CTA = 14 warps:
 //   warp 0       TMA producer (codes of both operands, weight scales)
-//   warp 1       MMA issuer: tcgen05.cp of a stage's scales into one of two
-//                TMEM buffers, then 4 x 2 MMAs
+//   warp 1       MMA issuer: 4 x 2 MMAs a stage
 //   warps 2-9    epilogue, two groups of four (warp w reads TMEM lanes
 //                32*(w%4)..+31 = its 32 weight rows; the groups alternate
-//                chunks of 16 tokens); each warp turns its 16 x 32 piece in
-//                shared memory so that a lane holds 16 consecutive outputs of
-//                one token: one 32-byte bf16 store, or one NVFP4 block
-//   warps 10-    activation scales, one warp for each ring slot: a warp that
-//                served several slots would not see every phase of their
-//                barriers, and a parity wait tells only neighbouring phases apart
+//                chunks of 16 tokens).  A warp first drains its part of the
+//                tile into registers as bf16 pairs of the two boxes (g and u,
+//                or columns c and c + 128) and gives the accumulator back,
+//                then turns each 16 x 32 piece in shared memory so that a lane
+//                holds 16 consecutive outputs of one token: one 32-byte bf16
+//                store, or one NVFP4 block
+//   warps 10-13  scales
 //
 // TMEM: columns 0..383 hold the accumulators (a unit of up to 96 token
 // columns takes half of them, so its epilogue overlaps the next unit's main
-// loop), 384..511 two buffers of scales (weights 2 boxes x 4 MMAs x 4 columns,
-// tokens 4 x 8).  A buffer is overwritten only after the MMAs that read it
-// have completed (the empty barrier of two stages before).
+// loop entirely), 384..511 two buffers of scales (weights 2 boxes x 4 MMAs x 4
+// columns, tokens 4 x 8).  A buffer is overwritten only after the MMAs that
+// read it have completed (the empty barrier of two stages before).
 //
 // Waits are bounded as in grouped_gemm.cu.
 #include <initializer_list>
@@ -68,7 +75,9 @@ constexpr int kBoxBytes = kBoxRows * kRowBytes;   // 16 KB
 constexpr int kSfTile = 512;                      // scales of 128 rows for one MMA
 constexpr int kSfBoxBytes = kSteps * kSfTile;     // 2 KB
 constexpr int kEpiWarps = 8;
+constexpr int kSfWarps = 4;                       // one for each lane quarter of TMEM
 constexpr int kFirstSfWarp = 2 + kEpiWarps;
+constexpr int kThreads = 32 * (kFirstSfWarp + kSfWarps);
 constexpr int kUnitQ = 4;                         // unit ids in flight between warps
 constexpr int kMaxExperts = 1024;
 constexpr int kAccCols = 192;                     // TMEM columns of an accumulator slot
@@ -82,26 +91,26 @@ template <int TOK, int STAGES, int MAX_E>
 struct Geom {
   static constexpr int kTok = TOK;
   static constexpr int kStages = STAGES;
-  static constexpr int kWarps = kFirstSfWarp + STAGES;  // a scale warp per ring slot
-  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kMaxE = MAX_E;
   static constexpr int kHalves = (TOK + 127) / 128;  // scale tiles of the tokens
   static constexpr int kTokBytes = TOK * kRowBytes;
-  static constexpr int kSfTokBytes = kSteps * kHalves * kSfTile;
+  static constexpr int kChunks = (TOK + 31) / 32;     // 16-token chunks of an epilogue group
+  static constexpr int kSfTokBytes = (TOK * 16 + 1023) / 1024 * 1024;
   static constexpr int kStageBytes = 2 * kBoxBytes + kTokBytes + 2 * kSfBoxBytes + kSfTokBytes;
   static_assert(TOK % 16 == 0 && TOK <= kAccCols, "a unit's tokens fit an accumulator slot");
   static_assert(kTokBytes % 1024 == 0 && kStageBytes % 1024 == 0, "swizzled boxes on 1 KB");
 };
 using GeomFull = Geom<192, 3, kMaxExperts>;
 // Every expert has at most 32 rows (decode): five stages in flight.
-using GeomDecode = Geom<32, 5, 256>;
+using GeomDecode = Geom<32, 5, kMaxExperts>;
 
 template <class G>
 struct SmemT {
   uint8_t ring[G::kStages][G::kStageBytes];  // 1024-byte aligned
   uint8_t turn[kEpiWarps][16 * kStagePitch];
-  uint64_t full_bar[G::kStages];   // TMA bytes + the scale warp
+  uint64_t full_bar[G::kStages];
   uint64_t empty_bar[G::kStages];
+  uint64_t sf_bar[2];             // a TMEM scale buffer is filled
   uint64_t acc_full_bar[2];
   uint64_t acc_empty_bar[2];
   uint64_t mma_done_bar;
@@ -110,7 +119,7 @@ struct SmemT {
   int32_t unit_q[kUnitQ];
   uint32_t tmem_base;
   int32_t abort;
-  int32_t warp_tot[G::kWarps];
+  int32_t warp_tot[kThreads / 32];
   int32_t offs[G::kMaxE + 1];
   int32_t cum[G::kMaxE + 1];
 };
@@ -145,7 +154,7 @@ struct Params {
   int n_out;
   float swiglu_limit;
   int32_t* counter;        // zeroed unit counter, or null (static stride)
-  int wide_scales;         // rows of a_sf are multiples of 16 bytes (K % 256 == 0)
+  int sf_by_tma;           // rows of a_sf are multiples of 16 bytes (K % 256 == 0)
 };
 
 // ---- PTX ----------------------------------------------------------------------
@@ -157,13 +166,35 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
-// 512 bytes of shared memory (32 rows of 16 bytes) -> 4 TMEM columns of 32
-// lanes, repeated in the four lane quarters.
-__device__ __forceinline__ void tmem_copy_sf(uint32_t taddr, uint32_t saddr) {
-  // no swizzle; 8-row groups 128 bytes apart, version 1 (sm_100)
-  const uint64_t desc = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) |
-                        (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0],"
+      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void umma_fp4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
                                          uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -221,16 +252,18 @@ __device__ __forceinline__ Unit decode_unit(const S& s, int num_experts, int id)
 }
 
 template <bool SWIGLU, class G>
-__global__ void __launch_bounds__(G::kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a64,
                     const __grid_constant__ CUtensorMap tmap_a16,
-                    const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ Params p) {
+                    const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ CUtensorMap tmap_s64,
+                    const __grid_constant__ CUtensorMap tmap_s16, const __grid_constant__ Params p) {
   using Smem = SmemT<G>;
   constexpr int S = G::kStages;
-  constexpr int kThreads = G::kThreads;
   constexpr int kTokOff = 2 * kBoxBytes;
   constexpr int kSfBOff = kTokOff + G::kTokBytes;       // weight scales
-  constexpr int kSfAOff = kSfBOff + 2 * kSfBoxBytes;    // token scales: tile (step, half)
+  constexpr int kSfAOff = kSfBOff + 2 * kSfBoxBytes;    // token scales, 16 bytes a row
+  constexpr int kSfTokCols = 4 * G::kHalves;            // TMEM columns of the tokens' scales of an MMA
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                      ~static_cast<uintptr_t>(1023));
@@ -272,17 +305,18 @@ __global__ void __launch_bounds__(G::kThreads, 1)
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&s.full_bar[i], 2);  // the producer's expect_tx and the scale warp
+      mbar_init(&s.full_bar[i], 1);
       mbar_init(&s.empty_bar[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.sf_bar[i], kSfWarps);
       mbar_init(&s.acc_full_bar[i], 1);
       mbar_init(&s.acc_empty_bar[i], kEpiWarps);
     }
     mbar_init(&s.mma_done_bar, 1);
     for (int i = 0; i < kUnitQ; ++i) {
       mbar_init(&s.q_full[i], 1);
-      mbar_init(&s.q_empty[i], 1 + kEpiWarps + S);
+      mbar_init(&s.q_empty[i], 1 + kEpiWarps + kSfWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a64)) : "memory");
@@ -347,7 +381,7 @@ __global__ void __launch_bounds__(G::kThreads, 1)
           uint8_t* st = s.ring[slot];
           uint64_t* full = &s.full_bar[slot];
           const uint32_t sf_bytes = min(kSteps, p.steps - kb * kSteps) * kSfTile;
-          mbar_expect_tx(full, nn * kRowBytes + boxes * (kBoxBytes + sf_bytes));
+          mbar_expect_tx(full, nn * (kRowBytes + (p.sf_by_tma ? 16 : 0)) + boxes * (kBoxBytes + sf_bytes));
           for (int b = 0; b < boxes; ++b) {
             tma_load_2d(st + b * kBoxBytes, &tmap_b, full, kb * kRowBytes, brow + b * p.b_second,
                         pol_w);
@@ -355,13 +389,15 @@ __global__ void __launch_bounds__(G::kThreads, 1)
                       sf + (static_cast<int64_t>(b * p.sf_second) * p.steps + kb * kSteps) * kSfTile,
                       sf_bytes, full);
           }
-          int r = 0;
-          for (; r + 64 <= nn; r += 64)
-            tma_load_2d(st + kTokOff + r * kRowBytes, &tmap_a64, full, kb * kRowBytes, u.row0 + r,
-                        pol_a);
-          for (; r < nn; r += 16)
-            tma_load_2d(st + kTokOff + r * kRowBytes, &tmap_a16, full, kb * kRowBytes, u.row0 + r,
-                        pol_a);
+          for (int r = 0; r < nn;) {
+            const bool big = r + 64 <= nn;
+            tma_load_2d(st + kTokOff + r * kRowBytes, big ? &tmap_a64 : &tmap_a16, full,
+                        kb * kRowBytes, u.row0 + r, pol_a);
+            if (p.sf_by_tma)
+              tma_load_2d(st + kSfAOff + r * 16, big ? &tmap_s64 : &tmap_s16, full, kb * 16,
+                          u.row0 + r, pol_a);
+            r += big ? 64 : 16;
+          }
         }
       }
       if (!ok) {  // let every issued load land before the CTA can exit
@@ -384,7 +420,6 @@ __global__ void __launch_bounds__(G::kThreads, 1)
         const Unit u = decode_unit<G>(s, E, unit);
         const int nn = (u.rows + 15) & ~15;
         const int boxes = boxes_of(u);
-        const int halves = nn > 128 ? 2 : 1;
         const uint32_t idesc = fp4_idesc(nn);
         const bool two = nn > kAccCols / 2;  // the unit takes both slots
         const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
@@ -401,13 +436,8 @@ __global__ void __launch_bounds__(G::kThreads, 1)
         const uint32_t d1 = d0 + (two ? kAccCols : kAccCols / 2);
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
           const int slot = j % S;
-          // The scale buffer was last read by the MMAs of two stages before.
-          if (j >= 2 && !mbar_wait(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u, abort,
-                                   kDevErrGemmMmaWait, true)) {
-            ok = false;
-            break;
-          }
-          if (!mbar_wait(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmMmaWait, true)) {
+          if (!mbar_wait(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmMmaWait, true) ||
+              !mbar_wait(&s.sf_bar[j & 1u], (j >> 1) & 1u, abort, kDevErrGemmMmaWait, true)) {
             ok = false;
             break;
           }
@@ -417,18 +447,13 @@ __global__ void __launch_bounds__(G::kThreads, 1)
           const uint32_t sft = sfb + 2 * kSteps * 4;                        // tokens
           const int steps = min(kSteps, p.steps - kb * kSteps);
           for (int k = 0; k < steps; ++k) {
-            for (int b = 0; b < boxes; ++b)
-              tmem_copy_sf(sfb + (k * 2 + b) * 4, st + kSfBOff + b * kSfBoxBytes + k * kSfTile);
-            for (int h = 0; h < halves; ++h)
-              tmem_copy_sf(sft + k * 8 + h * 4, st + kSfAOff + (k * G::kHalves + h) * kSfTile);
-          }
-          for (int k = 0; k < steps; ++k) {
             const uint64_t tok = smem_desc_sw128(st + kTokOff + k * 32);
             const uint32_t acc_in = (kb | k) != 0 ? 1u : 0u;
-            umma_fp4(d0, smem_desc_sw128(st + k * 32), tok, idesc, sfb + k * 8, sft + k * 8, acc_in);
+            umma_fp4(d0, smem_desc_sw128(st + k * 32), tok, idesc, sfb + k * 8,
+                     sft + k * kSfTokCols, acc_in);
             if (boxes == 2)
               umma_fp4(d1, smem_desc_sw128(st + kBoxBytes + k * 32), tok, idesc, sfb + k * 8 + 4,
-                       sft + k * 8, acc_in);
+                       sft + k * kSfTokCols, acc_in);
           }
           umma_commit(&s.empty_bar[slot]);
         }
@@ -442,9 +467,9 @@ __global__ void __launch_bounds__(G::kThreads, 1)
       mbar_wait(&s.mma_done_bar, 0, abort, kDevErrGemmMmaWait, false);
     }
   } else if (warp >= kFirstSfWarp) {
-    // ===================== activation scales (warps 10..) =====================
-    const uint32_t mine = static_cast<uint32_t>(warp - kFirstSfWarp);  // its ring slot
-    const int sf_row = p.steps * 4;  // scale bytes of a row
+    // ===================== scales (warps 10..13) =====================
+    const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;  // its TMEM lanes
+    const int sf_row = p.steps * 4;  // scale bytes of a token row
     uint32_t j = 0;
     bool ok = true;
     for (uint32_t qn = 0; ok; ++qn) {
@@ -457,51 +482,72 @@ __global__ void __launch_bounds__(G::kThreads, 1)
       if (lane == 0) mbar_arrive(&s.q_empty[qslot]);
       if (unit < 0) break;
       const Unit u = decode_unit<G>(s, E, unit);
-      const int halves = u.rows > 128 ? 2 : 1;
+      // Without TMA: the scales of stage kb of token row 32 q + lane, word k
+      // for MMA k.  Rows past the unit and MMAs past K get zeros.
+      auto load_tok = [&](int kb, uint32_t (&t)[4 * G::kHalves][kSteps]) {
+#pragma unroll
+        for (int q = 0; q < 4 * G::kHalves; ++q) {
+          const int r = q * 32 + lane;
+          const uint8_t* src = p.a_sf + static_cast<int64_t>(u.row0 + r) * sf_row + kb * (4 * kSteps);
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k)
+            t[q][k] = r < u.rows && kb * kSteps + k < p.steps
+                          ? __ldg(reinterpret_cast<const uint32_t*>(src) + k)
+                          : 0u;
+        }
+      };
+      uint32_t tok[4 * G::kHalves][kSteps];
       for (int kb = 0; kb < num_kb; ++kb, ++j) {
         const uint32_t slot = j % S;
-        if (slot != mine) continue;
-        const int steps = min(kSteps, p.steps - kb * kSteps);
-        // Row 32 q + lane of each half: its scales of the stage's four MMAs.
-        // Rows past the unit get zeros; their results are not stored.
-        uint32_t w[G::kHalves][4][kSteps];
-#pragma unroll
-        for (int h = 0; h < G::kHalves; ++h)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int r = h * 128 + q * 32 + lane;
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) w[h][q][k] = 0u;
-            if (r < u.rows) {
-              const uint8_t* src = p.a_sf + static_cast<int64_t>(u.row0 + r) * sf_row + kb * (4 * kSteps);
-              if (p.wide_scales) {
-                const uint4 v = ldg_nc_v4(src);
-                w[h][q][0] = v.x;
-                w[h][q][1] = v.y;
-                w[h][q][2] = v.z;
-                w[h][q][3] = v.w;
-              } else {
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-                  if (k < steps) w[h][q][k] = __ldg(reinterpret_cast<const uint32_t*>(src) + k);
-              }
-            }
-          }
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort,
-                                               kDevErrGemmScaleWait, true));
+        if (!p.sf_by_tma) load_tok(kb, tok);
+        // The stage has landed, and the MMAs of two stages before, which read
+        // this buffer, have completed.
+        bool got = mbar_wait(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmScaleWait, true);
+        if (j >= 2)
+          got = mbar_wait(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u, abort,
+                          kDevErrGemmScaleWait, true) && got;
+        ok = __all_sync(0xffffffffu, got);
         if (!ok) break;
-        uint8_t* dst = s.ring[slot] + kSfAOff + lane * 16;
+        tc_fence_after();
+        const uint32_t col = tmem_base + quarter + kSfCol + (j & 1u) * kSfBufCols;
+        const uint8_t* image = s.ring[slot] + kSfBOff + lane * 16;
+        uint32_t w[2 * kSteps * 4];
 #pragma unroll
-        for (int h = 0; h < G::kHalves; ++h)
-          if (h < halves)
+        for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-              *reinterpret_cast<uint4*>(dst + (k * G::kHalves + h) * kSfTile) =
-                  make_uint4(w[h][0][k], w[h][1][k], w[h][2][k], w[h][3][k]);
-        // Written by ordinary stores, read by tcgen05.cp through the async proxy.
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          for (int b = 0; b < 2; ++b) {
+            const uint4 v = *reinterpret_cast<const uint4*>(image + b * kSfBoxBytes + k * kSfTile);
+            w[(2 * k + b) * 4] = v.x;
+            w[(2 * k + b) * 4 + 1] = v.y;
+            w[(2 * k + b) * 4 + 2] = v.z;
+            w[(2 * k + b) * 4 + 3] = v.w;
+          }
+        tmem_st32(col, w);
+        if (p.sf_by_tma) {
+#pragma unroll
+          for (int q = 0; q < 4 * G::kHalves; ++q)
+            if (q * 32 < G::kTok) {
+              const uint4 v = *reinterpret_cast<const uint4*>(s.ring[slot] + kSfAOff + (q * 32 + lane) * 16);
+              tok[q][0] = v.x;
+              tok[q][1] = v.y;
+              tok[q][2] = v.z;
+              tok[q][3] = v.w;
+            }
+        }
+        uint32_t t[kSteps * kSfTokCols];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int q = 0; q < 4 * G::kHalves; ++q)
+            t[k * kSfTokCols + q] = q * 32 < G::kTok ? tok[q][k] : 0u;
+        if constexpr (G::kHalves == 2)
+          tmem_st32(col + 2 * kSteps * 4, t);
+        else
+          tmem_st16(col + 2 * kSteps * 4, t);
+        tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.full_bar[slot]);
+        if (lane == 0) mbar_arrive(&s.sf_bar[j & 1u]);
       }
     }
   } else {
@@ -542,27 +588,50 @@ __global__ void __launch_bounds__(G::kThreads, 1)
       const int tok = lane >> 1;                  // after the turn: token and
       const int feat = q * 32 + (lane & 1) * 16;  // first of 16 output columns of the box
       const uint4* mine = reinterpret_cast<const uint4*>(turn + tok * kStagePitch + (lane & 1) * 32);
-#pragma unroll 1
-      for (int t0 = grp * 16; t0 < nn; t0 += 32) {
-        uint32_t v0[16], v1[16];
-        tmem_ld16(d0 + t0, v0);
-        if (boxes == 2) tmem_ld16(d1 + t0, v1);
-        tmem_ld_wait();
+      // Drain: both boxes as a bf16 pair for each token of this warp's chunks.
+      uint32_t pair[G::kChunks][16];
+#pragma unroll
+      for (int c = 0; c < G::kChunks; ++c) {
+        const int t0 = (2 * c + grp) * 16;
+        if (t0 < nn) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+            uint32_t v0[8], v1[8];
+            tmem_ld8(d0 + t0 + i, v0);
+            tmem_ld8(d1 + t0 + i, v1);  // not written by a unit with one box; not used then
+            tmem_ld_wait();
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              pair[c][i + x] = pack_bf16x2(__fmul_rn(alpha, __uint_as_float(v0[x])),
+                                           __fmul_rn(alpha, __uint_as_float(v1[x])));
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&s.acc_empty_bar[acc0]);
+        if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
+      }
+#pragma unroll
+      for (int c = 0; c < G::kChunks; ++c) {
+        const int t0 = (2 * c + grp) * 16;
+        if (t0 >= nn) break;
         const int64_t row = u.row0 + t0 + tok;
         const bool live = t0 + tok < u.rows;
-#pragma unroll 1
-        for (int b = 0; b < (SWIGLU ? 1 : boxes); ++b) {
+#pragma unroll
+        for (int b = 0; b < (SWIGLU ? 1 : 2); ++b) {
+          if (b == 1 && boxes == 1) break;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            __nv_bfloat16 h;
-            if (SWIGLU) {
-              const float g = round_bf16(__fmul_rn(alpha, __uint_as_float(v0[i])));
-              const float up = round_bf16(__fmul_rn(alpha, __uint_as_float(v1[i])));
-              h = __float2bfloat16_rn(swiglu_f32(g, up, p.swiglu_limit));
-            } else {
-              h = __float2bfloat16_rn(__fmul_rn(alpha, __uint_as_float(b == 0 ? v0[i] : v1[i])));
-            }
-            *reinterpret_cast<__nv_bfloat16*>(turn + i * kStagePitch + lane * 2) = h;
+            uint16_t h;
+            if (SWIGLU)
+              h = __bfloat16_as_ushort(__float2bfloat16_rn(
+                  swiglu_f32(__uint_as_float(pair[c][i] << 16),
+                             __uint_as_float(pair[c][i] & 0xFFFF0000u), p.swiglu_limit)));
+            else
+              h = static_cast<uint16_t>(b == 0 ? pair[c][i] : pair[c][i] >> 16);
+            *reinterpret_cast<uint16_t*>(turn + i * kStagePitch + lane * 2) = h;
           }
           __syncwarp();
           const uint4 lo = mine[0], hi = mine[1];
@@ -582,12 +651,6 @@ __global__ void __launch_bounds__(G::kThreads, 1)
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&s.acc_empty_bar[acc0]);
-        if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
-      }
       ac += two ? 2u : 1u;
     }
   }
@@ -604,19 +667,21 @@ __global__ void __launch_bounds__(G::kThreads, 1)
 
 // ---- host side -----------------------------------------------------------------
 
-// 2-D byte map over a [outer, inner] row-major tensor, box [box_rows, 128 bytes],
-// 128-byte swizzle, zero fill out of bounds (code 0 = value 0).
+// 2-D byte map over a [outer, inner] row-major tensor, box [box_rows,
+// box_bytes], 128-byte swizzle for boxes of codes (128 bytes wide) and none for
+// scales (16 bytes), zero fill out of bounds (code 0 = value 0).
 lsek_status make_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
-                     uint32_t box_rows) {
+                     uint32_t box_rows, uint32_t box_bytes = kRowBytes) {
   EncodeTiledFn fn = tensor_map_encoder();
   if (fn == nullptr) return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: cuTensorMapEncodeTiled unavailable");
   const cuuint64_t dims[2] = {inner, outer};
   const cuuint64_t strides[1] = {inner};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(kRowBytes), box_rows};
+  const cuuint32_t box[2] = {box_bytes, box_rows};
   const cuuint32_t es[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
                         strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        box_bytes == kRowBytes ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
@@ -632,20 +697,25 @@ lsek_status launch_geom(Params p, const void* A, const void* B, int K, cudaStrea
                                 static_cast<int>(smem_bytes<G>()));
   });
   if (ae != cudaSuccess) return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: %s", cudaGetErrorString(ae));
-  CUtensorMap a64, a16, b;
+  CUtensorMap a64, a16, b, s64, s16;
   const uint64_t row_bytes = static_cast<uint64_t>(K) / 2;
   lsek_status s = make_map(&a64, A, row_bytes, static_cast<uint64_t>(p.rows), 64u);
   if (s == LSEK_OK) s = make_map(&a16, A, row_bytes, static_cast<uint64_t>(p.rows), 16u);
   if (s == LSEK_OK)
     s = make_map(&b, B, row_bytes, static_cast<uint64_t>(p.num_experts) * p.b_rows,
                  static_cast<uint32_t>(kBoxRows));
+  s64 = s16 = a16;  // unused without TMA
+  if (s == LSEK_OK && p.sf_by_tma) {
+    s = make_map(&s64, p.a_sf, row_bytes / 8, static_cast<uint64_t>(p.rows), 64u, 16u);
+    if (s == LSEK_OK) s = make_map(&s16, p.a_sf, row_bytes / 8, static_cast<uint64_t>(p.rows), 16u, 16u);
+  }
   if (s != LSEK_OK) return s;
   if (p.counter != nullptr) LSEK_CUDA_TRY(cudaMemsetAsync(p.counter, 0, sizeof(int32_t), st));
   // At most rows / kTok full chunks and one partial chunk per non-empty expert.
   const int64_t experts = p.num_experts < p.rows ? p.num_experts : p.rows;
   const int64_t max_units = (p.rows / G::kTok + experts) * static_cast<int64_t>(p.n_tiles);
   const int grid = static_cast<int>(max_units < num_sms() ? max_units : num_sms());
-  fp4_gemm_kernel<SWIGLU, G><<<grid, G::kThreads, smem_bytes<G>(), st>>>(a64, a16, b, p);
+  fp4_gemm_kernel<SWIGLU, G><<<grid, kThreads, smem_bytes<G>(), st>>>(a64, a16, b, s64, s16, p);
   return check_launch(SWIGLU ? "grouped_gemm_swiglu_nvfp4" : "grouped_gemm_nvfp4");
 }
 
@@ -685,7 +755,7 @@ lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales
   p.n_out = n_out;
   p.swiglu_limit = limit;
   p.counter = counter;
-  p.wide_scales = K % (kSteps * kStepK) == 0;
+  p.sf_by_tma = K % (kSteps * kStepK) == 0;
   const int col_tiles = static_cast<int>(ceil_div(n_out, kBoxRows));
   if (swiglu) {  // gate rows and up rows are tiled apart
     p.b_rows = 2 * n_out;
@@ -706,7 +776,7 @@ lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales
   }
   p.n_tiles = static_cast<int>(ceil_div(n_out, p.out_tile_cols));
   const int bound = max_rows_per_expert >= 0 && max_rows_per_expert < rows ? max_rows_per_expert : rows;
-  if (bound <= GeomDecode::kTok && E <= GeomDecode::kMaxE)
+  if (bound <= GeomDecode::kTok)
     return swiglu ? launch_geom<true, GeomDecode>(p, A, B, K, st)
                   : launch_geom<false, GeomDecode>(p, A, B, K, st);
   return swiglu ? launch_geom<true, GeomFull>(p, A, B, K, st)
