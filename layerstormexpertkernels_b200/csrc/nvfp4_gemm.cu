@@ -38,8 +38,8 @@
 // to 16 of them a stage, in line with the MMAs: 1.5 times the whole kernel's
 // time (64 experts, H=7168, I=2048: 270 against 183 us at one row an expert).
 //
-// One CTA = 14 warps:
-//   warp 0       TMA producer (codes of both operands, weight scales)
+// One CTA = 16 warps:
+//   warp 0       takes units; TMA producer of the weights' codes
 //   warp 1       MMA issuer: 4 x 2 MMAs a stage
 //   warps 2-9    epilogue, two groups of four (warp w reads TMEM lanes
 //                32*(w%4)..+31 = its 32 weight rows; the groups alternate
@@ -49,7 +49,10 @@
 //                then turns each 16 x 32 piece in shared memory so that a lane
 //                holds 16 consecutive outputs of one token: one 32-byte bf16
 //                store, or one NVFP4 block
-//   warps 10-13  scales
+//   warps 10-13  scales: shared memory -> TMEM
+//   warp 14      TMA producer of the tokens' codes
+//   warp 15      TMA producer of scales, into a ring of their own: they are in
+//                TMEM by the time the codes land
 //
 // TMEM: columns 0..383 hold the accumulators (a unit of up to 96 token
 // columns takes half of them, so its epilogue overlaps the next unit's main
@@ -77,7 +80,9 @@ constexpr int kSfBoxBytes = kSteps * kSfTile;     // 2 KB
 constexpr int kEpiWarps = 8;
 constexpr int kSfWarps = 4;                       // one for each lane quarter of TMEM
 constexpr int kFirstSfWarp = 2 + kEpiWarps;
-constexpr int kThreads = 32 * (kFirstSfWarp + kSfWarps);
+constexpr int kTokWarp = kFirstSfWarp + kSfWarps; // TMA producer of the tokens' codes
+constexpr int kSfLoadWarp = kTokWarp + 1;         // TMA producer of scales
+constexpr int kThreads = 32 * (kSfLoadWarp + 1);
 constexpr int kUnitQ = 4;                         // unit ids in flight between warps
 constexpr int kMaxExperts = 1024;
 constexpr int kAccCols = 192;                     // TMEM columns of an accumulator slot
@@ -87,29 +92,33 @@ constexpr int kTmemCols = 512;
 constexpr int kStagePitch = 80;                   // epilogue: bytes of a token's 32 bf16 (+ pad)
 
 // TOK: most token rows of a unit; MAX_E: experts that the unit table holds.
-template <int TOK, int STAGES, int MAX_E>
+template <int TOK, int STAGES, int SF_STAGES, int MAX_E>
 struct Geom {
   static constexpr int kTok = TOK;
-  static constexpr int kStages = STAGES;
+  static constexpr int kStages = STAGES;       // of codes
+  static constexpr int kSfStages = SF_STAGES;  // of scales
   static constexpr int kMaxE = MAX_E;
   static constexpr int kHalves = (TOK + 127) / 128;  // scale tiles of the tokens
   static constexpr int kTokBytes = TOK * kRowBytes;
   static constexpr int kChunks = (TOK + 31) / 32;     // 16-token chunks of an epilogue group
-  static constexpr int kSfTokBytes = (TOK * 16 + 1023) / 1024 * 1024;
-  static constexpr int kStageBytes = 2 * kBoxBytes + kTokBytes + 2 * kSfBoxBytes + kSfTokBytes;
+  static constexpr int kStageBytes = 2 * kBoxBytes + kTokBytes;
+  static constexpr int kSfStageBytes = 2 * kSfBoxBytes + TOK * 16;
   static_assert(TOK % 16 == 0 && TOK <= kAccCols, "a unit's tokens fit an accumulator slot");
   static_assert(kTokBytes % 1024 == 0 && kStageBytes % 1024 == 0, "swizzled boxes on 1 KB");
 };
-using GeomFull = Geom<192, 3, kMaxExperts>;
+using GeomFull = Geom<192, 3, 4, kMaxExperts>;
 // Every expert has at most 32 rows (decode): five stages in flight.
-using GeomDecode = Geom<32, 5, kMaxExperts>;
+using GeomDecode = Geom<32, 5, 5, kMaxExperts>;
 
 template <class G>
 struct SmemT {
   uint8_t ring[G::kStages][G::kStageBytes];  // 1024-byte aligned
+  uint8_t sf_ring[G::kSfStages][G::kSfStageBytes];
   uint8_t turn[kEpiWarps][16 * kStagePitch];
   uint64_t full_bar[G::kStages];
   uint64_t empty_bar[G::kStages];
+  uint64_t sf_full_bar[G::kSfStages];
+  uint64_t sf_empty_bar[G::kSfStages];
   uint64_t sf_bar[2];             // a TMEM scale buffer is filled
   uint64_t acc_full_bar[2];
   uint64_t acc_empty_bar[2];
@@ -270,9 +279,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap tmap_s16, const __grid_constant__ Params p) {
   using Smem = SmemT<G>;
   constexpr int S = G::kStages;
+  constexpr int SS = G::kSfStages;
   constexpr int kTokOff = 2 * kBoxBytes;
-  constexpr int kSfBOff = kTokOff + G::kTokBytes;       // weight scales
-  constexpr int kSfAOff = kSfBOff + 2 * kSfBoxBytes;    // token scales, 16 bytes a row
+  constexpr int kSfTokOff = 2 * kSfBoxBytes;            // token scales, 16 bytes a row
   constexpr int kSfTokCols = 4 * G::kHalves;            // TMEM columns of the tokens' scales of an MMA
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -315,8 +324,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&s.full_bar[i], 1);
+      mbar_init(&s.full_bar[i], 2);  // both producers of codes
       mbar_init(&s.empty_bar[i], 1);
+    }
+    for (int i = 0; i < SS; ++i) {
+      mbar_init(&s.sf_full_bar[i], 1);
+      mbar_init(&s.sf_empty_bar[i], kSfWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.sf_bar[i], kSfWarps);
@@ -326,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&s.mma_done_bar, 1);
     for (int i = 0; i < kUnitQ; ++i) {
       mbar_init(&s.q_full[i], 1);
-      mbar_init(&s.q_empty[i], 1 + kEpiWarps + kSfWarps);
+      mbar_init(&s.q_empty[i], 1 + kEpiWarps + kSfWarps + 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a64)) : "memory");
@@ -354,65 +367,134 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto boxes_of = [&](const Unit& u) { return SWIGLU || cols_of(u) > kBoxRows ? 2 : 1; };
 
   if (warp == 0) {
-    // ===================== TMA producer =====================
+    // ===================== units; TMA producer of the weights' codes =====================
     if (elect_one()) {
-      // Weights: normal eviction, so the other chunks of an expert find them
-      // in L2; tokens are read by every n-tile and stay.
-      const uint64_t pol_w = policy_evict_normal();
-      const uint64_t pol_a = policy_evict_last();
+      // Normal eviction: the other chunks of an expert find the weights in L2.
+      const uint64_t policy = policy_evict_normal();
       bool ok = true;
       uint32_t j = 0;  // stages issued so far
-      uint32_t qn = 0;
-      for (int i = 0; ok; ++i, ++qn) {
+      for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
         if (!mbar_wait(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort,
                        kDevErrGemmProducerWait, true)) {
           ok = false;
           break;
         }
-        int unit = p.counter ? atomicAdd(p.counter, 1) : blockIdx.x + i * static_cast<int>(gridDim.x);
+        int unit = p.counter ? atomicAdd(p.counter, 1)
+                             : static_cast<int>(blockIdx.x + qn * gridDim.x);
         if (unit >= total) unit = -1;
         s.unit_q[qslot] = unit;
         mbar_arrive(&s.q_full[qslot]);
         if (unit < 0) break;
         const Unit u = decode_unit<G>(s, E, unit);
-        const int nn = (u.rows + 15) & ~15;
         const int boxes = boxes_of(u);
         const int brow = u.e * p.b_rows + u.n * p.b_tile_rows;
-        const uint8_t* sf = p.b_sf + static_cast<int64_t>(u.e * p.sf_tiles + u.n * p.sf_tile_step) *
-                                         p.steps * kSfTile;
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
-          const int slot = j % S;
+          const uint32_t slot = j % S;
           if (!mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait,
                          true)) {
             ok = false;
             break;
           }
-          uint8_t* st = s.ring[slot];
-          uint64_t* full = &s.full_bar[slot];
-          const uint32_t sf_bytes = min(kSteps, p.steps - kb * kSteps) * kSfTile;
-          mbar_expect_tx(full, nn * (kRowBytes + (p.sf_by_tma ? 16 : 0)) + boxes * (kBoxBytes + sf_bytes));
-          for (int b = 0; b < boxes; ++b) {
-            tma_load_2d(st + b * kBoxBytes, &tmap_b, full, kb * kRowBytes, brow + b * p.b_second,
-                        pol_w);
-            bulk_load(st + kSfBOff + b * kSfBoxBytes,
-                      sf + (static_cast<int64_t>(b * p.sf_second) * p.steps + kb * kSteps) * kSfTile,
-                      sf_bytes, full);
-          }
-          for (int r = 0; r < nn;) {
-            const bool big = r + 64 <= nn;
-            tma_load_2d(st + kTokOff + r * kRowBytes, big ? &tmap_a64 : &tmap_a16, full,
-                        kb * kRowBytes, u.row0 + r, pol_a);
-            if (p.sf_by_tma)
-              tma_load_2d(st + kSfAOff + r * 16, big ? &tmap_s64 : &tmap_s16, full, kb * 16,
-                          u.row0 + r, pol_a);
-            r += big ? 64 : 16;
-          }
+          mbar_expect_tx(&s.full_bar[slot], boxes * kBoxBytes);
+          tma_load_2d(s.ring[slot], &tmap_b, &s.full_bar[slot], kb * kRowBytes, brow, policy);
+          if (boxes == 2)
+            tma_load_2d(s.ring[slot] + kBoxBytes, &tmap_b, &s.full_bar[slot], kb * kRowBytes,
+                        brow + p.b_second, policy);
         }
       }
       if (!ok) {  // let every issued load land before the CTA can exit
         for (uint32_t d = j > S ? j - S : 0; d < j; ++d)
           mbar_wait(&s.full_bar[d % S], (d / S) & 1u, abort, kDevErrGemmProducerWait, false);
+      }
+    }
+  } else if (warp == kTokWarp) {
+    // ===================== TMA producer of the tokens' codes =====================
+    if (elect_one()) {
+      const uint64_t policy = policy_evict_last();  // read by every n-tile
+      bool ok = true;
+      uint32_t j = 0;
+      for (uint32_t qn = 0; ok; ++qn) {
+        const int qslot = qn % kUnitQ;
+        if (!mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmProducerWait, true)) {
+          ok = false;
+          break;
+        }
+        const int unit = s.unit_q[qslot];
+        mbar_arrive(&s.q_empty[qslot]);
+        if (unit < 0) break;
+        const Unit u = decode_unit<G>(s, E, unit);
+        const int nn = (u.rows + 15) & ~15;
+        for (int kb = 0; kb < num_kb; ++kb, ++j) {
+          const uint32_t slot = j % S;
+          if (!mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait,
+                         true)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&s.full_bar[slot], nn * kRowBytes);
+          for (int r = 0; r < nn;) {
+            const bool big = r + 64 <= nn;
+            tma_load_2d(s.ring[slot] + kTokOff + r * kRowBytes, big ? &tmap_a64 : &tmap_a16,
+                        &s.full_bar[slot], kb * kRowBytes, u.row0 + r, policy);
+            r += big ? 64 : 16;
+          }
+        }
+      }
+      if (!ok) {
+        for (uint32_t d = j > S ? j - S : 0; d < j; ++d)
+          mbar_wait(&s.full_bar[d % S], (d / S) & 1u, abort, kDevErrGemmProducerWait, false);
+      }
+    }
+  } else if (warp == kSfLoadWarp) {
+    // ===================== TMA producer of scales =====================
+    // Runs up to SS stages ahead of the scale warps, which release a slot as
+    // soon as they have read it, so scales wait in TMEM before their codes land.
+    if (elect_one()) {
+      const uint64_t policy = policy_evict_last();
+      bool ok = true;
+      uint32_t j = 0;
+      for (uint32_t qn = 0; ok; ++qn) {
+        const int qslot = qn % kUnitQ;
+        if (!mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmScaleWait, true)) {
+          ok = false;
+          break;
+        }
+        const int unit = s.unit_q[qslot];
+        mbar_arrive(&s.q_empty[qslot]);
+        if (unit < 0) break;
+        const Unit u = decode_unit<G>(s, E, unit);
+        const int nn = (u.rows + 15) & ~15;
+        const int boxes = boxes_of(u);
+        const uint8_t* sf = p.b_sf + static_cast<int64_t>(u.e * p.sf_tiles + u.n * p.sf_tile_step) *
+                                         p.steps * kSfTile;
+        const uint8_t* sf2 = sf + static_cast<int64_t>(p.sf_second) * p.steps * kSfTile;
+        for (int kb = 0; kb < num_kb; ++kb, ++j) {
+          const uint32_t slot = j % SS;
+          if (!mbar_wait(&s.sf_empty_bar[slot], ((j / SS) & 1u) ^ 1u, abort, kDevErrGemmScaleWait,
+                         true)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = s.sf_ring[slot];
+          uint64_t* full = &s.sf_full_bar[slot];
+          const uint32_t bytes = min(kSteps, p.steps - kb * kSteps) * kSfTile;
+          mbar_expect_tx(full, boxes * bytes + (p.sf_by_tma ? nn * 16 : 0));
+          bulk_load(st, sf + kb * kSfBoxBytes, bytes, full);
+          if (boxes == 2) bulk_load(st + kSfBoxBytes, sf2 + kb * kSfBoxBytes, bytes, full);
+          if (p.sf_by_tma) {
+            for (int r = 0; r < nn;) {
+              const bool big = r + 64 <= nn;
+              tma_load_2d(st + kSfTokOff + r * 16, big ? &tmap_s64 : &tmap_s16, full, kb * 16,
+                          u.row0 + r, policy);
+              r += big ? 64 : 16;
+            }
+          }
+        }
+      }
+      if (!ok) {
+        for (uint32_t d = j > SS ? j - SS : 0; d < j; ++d)
+          mbar_wait(&s.sf_full_bar[d % SS], (d / SS) & 1u, abort, kDevErrGemmScaleWait, false);
       }
     }
   } else if (warp == 1) {
@@ -476,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(&s.mma_done_bar);
       mbar_wait(&s.mma_done_bar, 0, abort, kDevErrGemmMmaWait, false);
     }
-  } else if (warp >= kFirstSfWarp) {
+  } else if (warp >= kFirstSfWarp && warp < kTokWarp) {
     // ===================== scales (warps 10..13) =====================
     const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;  // its TMEM lanes
     const int sf_row = p.steps * 4;  // scale bytes of a token row
@@ -508,19 +590,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       uint32_t tok[4 * G::kHalves][kSteps];
       for (int kb = 0; kb < num_kb; ++kb, ++j) {
-        const uint32_t slot = j % S;
+        const uint32_t slot = j % SS;
         if (!p.sf_by_tma) load_tok(kb, tok);
-        // The stage has landed, and the MMAs of two stages before, which read
-        // this buffer, have completed.
-        bool got = mbar_wait(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmScaleWait, true);
-        if (j >= 2)
-          got = mbar_wait(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u, abort,
-                          kDevErrGemmScaleWait, true) && got;
-        ok = __all_sync(0xffffffffu, got);
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.sf_full_bar[slot], (j / SS) & 1u, abort,
+                                               kDevErrGemmScaleWait, true));
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t col = tmem_base + quarter + kSfCol + (j & 1u) * kSfBufCols;
-        const uint8_t* image = s.ring[slot] + kSfBOff + lane * 16;
+        const uint8_t* image = s.sf_ring[slot] + lane * 16;
         uint32_t w[2 * kSteps * 4];
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
@@ -532,12 +607,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             w[(2 * k + b) * 4 + 2] = v.z;
             w[(2 * k + b) * 4 + 3] = v.w;
           }
-        tmem_st32(col, w);
         if (p.sf_by_tma) {
 #pragma unroll
           for (int q = 0; q < 4 * G::kHalves; ++q)
             if (q * 32 < G::kTok) {
-              const uint4 v = *reinterpret_cast<const uint4*>(s.ring[slot] + kSfAOff + (q * 32 + lane) * 16);
+              const uint4 v = *reinterpret_cast<const uint4*>(image + kSfTokOff + q * 512);
               tok[q][0] = v.x;
               tok[q][1] = v.y;
               tok[q][2] = v.z;
@@ -550,6 +624,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int q = 0; q < 4 * G::kHalves; ++q)
             t[k * kSfTokCols + q] = q * 32 < G::kTok ? tok[q][k] : 0u;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.sf_empty_bar[slot]);
+        // The MMAs of two stages before, which read this buffer, have completed.
+        if (j >= 2)
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u,
+                                                 abort, kDevErrGemmScaleWait, true));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t col = tmem_base + quarter + kSfCol + (j & 1u) * kSfBufCols;
+        tmem_st32(col, w);
         if constexpr (G::kHalves == 2)
           tmem_st32(col + 2 * kSteps * 4, t);
         else
