@@ -168,6 +168,13 @@ struct Params {
 
 // ---- PTX ----------------------------------------------------------------------
 
+// mbar_wait with its first try inline: the call alone costs hundreds of cycles
+// in a chain that has a wait in every link.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int32_t* abort,
+                                         int32_t code) {
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort, code, true);
+}
+
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -375,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t j = 0;  // stages issued so far
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
-        if (!mbar_wait(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort,
-                       kDevErrGemmProducerWait, true)) {
+        if (!wait_bar(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort,
+                       kDevErrGemmProducerWait)) {
           ok = false;
           break;
         }
@@ -391,8 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int brow = u.e * p.b_rows + u.n * p.b_tile_rows;
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
           const uint32_t slot = j % S;
-          if (!mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait,
-                         true)) {
+          if (!wait_bar(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait)) {
             ok = false;
             break;
           }
@@ -416,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t j = 0;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
-        if (!mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmProducerWait, true)) {
+        if (!wait_bar(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmProducerWait)) {
           ok = false;
           break;
         }
@@ -427,8 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nn = (u.rows + 15) & ~15;
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
           const uint32_t slot = j % S;
-          if (!mbar_wait(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait,
-                         true)) {
+          if (!wait_bar(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait)) {
             ok = false;
             break;
           }
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t j = 0;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
-        if (!mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmScaleWait, true)) {
+        if (!wait_bar(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmScaleWait)) {
           ok = false;
           break;
         }
@@ -471,8 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* sf2 = sf + static_cast<int64_t>(p.sf_second) * p.steps * kSfTile;
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
           const uint32_t slot = j % SS;
-          if (!mbar_wait(&s.sf_empty_bar[slot], ((j / SS) & 1u) ^ 1u, abort, kDevErrGemmScaleWait,
-                         true)) {
+          if (!wait_bar(&s.sf_empty_bar[slot], ((j / SS) & 1u) ^ 1u, abort, kDevErrGemmScaleWait)) {
             ok = false;
             break;
           }
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
-        if (!mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmMmaWait, true)) break;
+        if (!wait_bar(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmMmaWait)) break;
         const int unit = s.unit_q[qslot];
         mbar_arrive(&s.q_empty[qslot]);
         if (unit < 0) break;
@@ -515,8 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t idesc = fp4_idesc(nn);
         const bool two = nn > kAccCols / 2;  // the unit takes both slots
         const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
-        if (!mbar_wait(&s.acc_empty_bar[acc0], ((ac >> 1) & 1u) ^ 1u, abort, kDevErrGemmMmaWait,
-                       true) ||
+        if (!wait_bar(&s.acc_empty_bar[acc0], ((ac >> 1) & 1u) ^ 1u, abort, kDevErrGemmMmaWait) ||
             (two && !mbar_wait(&s.acc_empty_bar[acc1], (((ac + 1) >> 1) & 1u) ^ 1u, abort,
                                kDevErrGemmMmaWait, true))) {
           ok = false;
@@ -528,8 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t d1 = d0 + (two ? kAccCols : kAccCols / 2);
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
           const int slot = j % S;
-          if (!mbar_wait(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmMmaWait, true) ||
-              !mbar_wait(&s.sf_bar[j & 1u], (j >> 1) & 1u, abort, kDevErrGemmMmaWait, true)) {
+          if (!wait_bar(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmMmaWait) ||
+              !wait_bar(&s.sf_bar[j & 1u], (j >> 1) & 1u, abort, kDevErrGemmMmaWait)) {
             ok = false;
             break;
           }
@@ -566,8 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (uint32_t qn = 0; ok; ++qn) {
       const int qslot = qn % kUnitQ;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort,
-                                             kDevErrGemmScaleWait, true));
+      ok = __all_sync(0xffffffffu, wait_bar(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort,
+                                             kDevErrGemmScaleWait));
       if (!ok) break;
       const int unit = s.unit_q[qslot];
       __syncwarp();
@@ -592,8 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int kb = 0; kb < num_kb; ++kb, ++j) {
         const uint32_t slot = j % SS;
         if (!p.sf_by_tma) load_tok(kb, tok);
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.sf_full_bar[slot], (j / SS) & 1u, abort,
-                                               kDevErrGemmScaleWait, true));
+        ok = __all_sync(0xffffffffu, wait_bar(&s.sf_full_bar[slot], (j / SS) & 1u, abort,
+                                               kDevErrGemmScaleWait));
         if (!ok) break;
         const uint8_t* image = s.sf_ring[slot] + lane * 16;
         uint32_t w[2 * kSteps * 4];
@@ -628,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&s.sf_empty_bar[slot]);
         // The MMAs of two stages before, which read this buffer, have completed.
         if (j >= 2)
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u,
-                                                 abort, kDevErrGemmScaleWait, true));
+          ok = __all_sync(0xffffffffu, wait_bar(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u,
+                                                 abort, kDevErrGemmScaleWait));
         if (!ok) break;
         tc_fence_after();
         const uint32_t col = tmem_base + quarter + kSfCol + (j & 1u) * kSfBufCols;
@@ -655,8 +658,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t ac = 0;
     for (uint32_t qn = 0;; ++qn) {
       const int qslot = qn % kUnitQ;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort,
-                                             kDevErrGemmEpilogueWait, true)))
+      if (!__all_sync(0xffffffffu, wait_bar(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort,
+                                             kDevErrGemmEpilogueWait)))
         break;
       const int unit = s.unit_q[qslot];
       __syncwarp();
@@ -666,10 +669,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nn = (u.rows + 15) & ~15;
       const bool two = nn > kAccCols / 2;
       const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
-      bool got = mbar_wait(&s.acc_full_bar[acc0], (ac >> 1) & 1u, abort, kDevErrGemmEpilogueWait, true);
+      bool got = wait_bar(&s.acc_full_bar[acc0], (ac >> 1) & 1u, abort, kDevErrGemmEpilogueWait);
       if (two)
-        got = mbar_wait(&s.acc_full_bar[acc1], ((ac + 1) >> 1) & 1u, abort, kDevErrGemmEpilogueWait,
-                        true) && got;
+        got = wait_bar(&s.acc_full_bar[acc1], ((ac + 1) >> 1) & 1u, abort, kDevErrGemmEpilogueWait) && got;
       if (!__all_sync(0xffffffffu, got)) break;
       tc_fence_after();
       const uint32_t d0 = tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
