@@ -41,8 +41,7 @@ lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales
                              const void* a_scales, const void* B, const void* b_tiles,
                              const int32_t* offsets, const float* a_global, const float* b_global,
                              const float* out_global, int E, int rows, int n_out, int K,
-                             float limit, int32_t* counter, cudaStream_t st,
-                             int max_rows_per_expert);
+                             float limit, int32_t* counter, cudaStream_t st);
 
 namespace {
 struct LayerWs {
@@ -256,16 +255,14 @@ extern "C" lsek_status lsek_moe_layer_forward_nvfp4(
                               hidden_dim, st);
   if (s != LSEK_OK) return s;
   if ((s = mark(3)) != LSEK_OK) return s;
-  // The top-k experts of a token are distinct, so no expert gets more than T rows.
   s = grouped_gemm_fp4(true, nullptr, ws + l.h, ws + l.hs, ws + l.x, ws + l.xs, W_gu,
                        gu_scale_tiles, offs, hidden_global_scale, gu_global_scale,
-                       inter_global_scale, E, rows, inter_dim, hidden_dim, swiglu_limit, counter,
-                       st, T);
+                       inter_global_scale, E, rows, inter_dim, hidden_dim, swiglu_limit, counter, st);
   if (s != LSEK_OK) return s;
   if ((s = mark(4)) != LSEK_OK) return s;
   s = grouped_gemm_fp4(false, ws + l.y, nullptr, nullptr, ws + l.h, ws + l.hs, W_down,
                        down_scale_tiles, offs, inter_global_scale, down_global_scale, nullptr, E,
-                       rows, hidden_dim, inter_dim, 0.0f, counter, st, T);
+                       rows, hidden_dim, inter_dim, 0.0f, counter, st);
   if (s != LSEK_OK) return s;
   if ((s = mark(5)) != LSEK_OK) return s;
   s = lsek_moe_unpermute(out, ws + l.y, w, s2d, T, k, hidden_dim, LSEK_BF16, 0, stream);

@@ -91,34 +91,68 @@ constexpr int kSfBufCols = 64;
 constexpr int kTmemCols = 512;
 constexpr int kStagePitch = 80;                   // epilogue: bytes of a token's 32 bf16 (+ pad)
 
-// TOK: most token rows of a unit; MAX_E: experts that the unit table holds.
-template <int TOK, int STAGES, int SF_STAGES, int MAX_E>
+constexpr int kTok = 192;                         // most token rows of a unit
+constexpr int kHalves = 2;                        // 128-row scale tiles of the tokens
+constexpr int kChunks = kTok / 32;                // 16-token chunks of an epilogue group
+constexpr int kRecs = 8;                          // stages in flight at most
+constexpr int kSfStages = 3;
+constexpr int kSfTokOff = 2 * kSfBoxBytes;        // token scales, 16 bytes a row
+constexpr int kSfStageBytes = kSfTokOff + kTok * 16;
+
+// The ring of codes is given out in bytes: a stage takes its two weight boxes
+// (16 KB each) and 128 bytes for each token row, so that a decode batch has
+// five stages in flight and an expert of 144 rows nearly four.  RING is what
+// shared memory leaves beside the unit table of MAX_E experts.
+template <int RING, int MAX_E>
 struct Geom {
-  static constexpr int kTok = TOK;
-  static constexpr int kStages = STAGES;       // of codes
-  static constexpr int kSfStages = SF_STAGES;  // of scales
+  static constexpr uint32_t kRing = RING;
   static constexpr int kMaxE = MAX_E;
-  static constexpr int kHalves = (TOK + 127) / 128;  // scale tiles of the tokens
-  static constexpr int kTokBytes = TOK * kRowBytes;
-  static constexpr int kChunks = (TOK + 31) / 32;     // 16-token chunks of an epilogue group
-  static constexpr int kStageBytes = 2 * kBoxBytes + kTokBytes;
-  static constexpr int kSfStageBytes = 2 * kSfBoxBytes + TOK * 16;
-  static_assert(TOK % 16 == 0 && TOK <= kAccCols, "a unit's tokens fit an accumulator slot");
-  static_assert(kTokBytes % 1024 == 0 && kStageBytes % 1024 == 0, "swizzled boxes on 1 KB");
+  static_assert(RING % 1024 == 0, "swizzled boxes start on 1 KB");
+  static_assert(RING >= 2 * (2 * kBoxBytes + kTok * kRowBytes), "two of the largest stages fit");
 };
-using GeomFull = Geom<192, 3, 4, kMaxExperts>;
-// Every expert has at most 32 rows (decode): five stages in flight.
-using GeomDecode = Geom<32, 5, 5, kMaxExperts>;
+using GeomFull = Geom<192 * 1024, 256>;
+using GeomWide = Geom<184 * 1024, kMaxExperts>;
+
+// Position in the ring.  Every role walks the same stages and keeps its own
+// copy; stage j uses record j % kRecs (parity (j / kRecs) & 1).
+template <class G>
+struct RingPos {
+  uint32_t j = 0;    // stages so far
+  uint32_t off = 0;  // where the next part goes
+  uint32_t w0, w1, tok;  // parts of the current stage
+  __device__ __forceinline__ int rec() const { return static_cast<int>(j % kRecs); }
+  __device__ __forceinline__ uint32_t parity() const { return (j / kRecs) & 1u; }
+  // Lays the next stage out: its boxes of weights and its token rows, each in
+  // one piece; a piece that would cross the ring's end starts at 0 instead.
+  // Returns the bytes taken, skipped ones included.
+  __device__ __forceinline__ uint32_t layout(int boxes, uint32_t tok_bytes) {
+    uint32_t span = 0;
+    auto place = [&](uint32_t size) -> uint32_t {
+      if (off + size > G::kRing) {
+        span += G::kRing - off;
+        off = 0;
+      }
+      const uint32_t at = off;
+      off += size;
+      span += size;
+      return at;
+    };
+    w0 = place(kBoxBytes);
+    w1 = boxes == 2 ? place(kBoxBytes) : 0u;
+    tok = place(tok_bytes);
+    return span;
+  }
+};
 
 template <class G>
 struct SmemT {
-  uint8_t ring[G::kStages][G::kStageBytes];  // 1024-byte aligned
-  uint8_t sf_ring[G::kSfStages][G::kSfStageBytes];
+  uint8_t ring[G::kRing];  // 1024-byte aligned
+  uint8_t sf_ring[kSfStages][kSfStageBytes];
   uint8_t turn[kEpiWarps][16 * kStagePitch];
-  uint64_t full_bar[G::kStages];
-  uint64_t empty_bar[G::kStages];
-  uint64_t sf_full_bar[G::kSfStages];
-  uint64_t sf_empty_bar[G::kSfStages];
+  uint64_t full_bar[kRecs];
+  uint64_t empty_bar[kRecs];
+  uint64_t sf_full_bar[kSfStages];
+  uint64_t sf_empty_bar[kSfStages];
   uint64_t sf_bar[2];             // a TMEM scale buffer is filled
   uint64_t acc_full_bar[2];
   uint64_t acc_empty_bar[2];
@@ -126,6 +160,7 @@ struct SmemT {
   uint64_t q_full[kUnitQ];
   uint64_t q_empty[kUnitQ];
   int32_t unit_q[kUnitQ];
+  uint32_t span[2][kRecs];  // ring bytes of each outstanding stage, for each producer of codes
   uint32_t tmem_base;
   int32_t abort;
   int32_t warp_tot[kThreads / 32];
@@ -137,7 +172,7 @@ constexpr size_t smem_bytes() {
   return sizeof(SmemT<G>) + 1024;
 }
 static_assert(smem_bytes<GeomFull>() <= 227 * 1024, "shared memory budget");
-static_assert(smem_bytes<GeomDecode>() <= 227 * 1024, "shared memory budget");
+static_assert(smem_bytes<GeomWide>() <= 227 * 1024, "shared memory budget");
 
 struct Params {
   const int32_t* offsets;  // [E+1]
@@ -166,6 +201,13 @@ struct Params {
   int sf_by_tma;           // rows of a_sf are multiples of 16 bytes (K % 256 == 0)
 };
 
+// Tensor maps: weights in boxes of 128 rows; tokens and their scales in boxes of
+// 16 << i rows, so that any multiple of 16 up to 192 takes at most four loads
+// (each costs its lane about 50 cycles).
+struct Maps {
+  CUtensorMap b, a[4], s[4];
+};
+
 // ---- PTX ----------------------------------------------------------------------
 
 // mbar_wait with its first try inline: the call alone costs hundreds of cycles
@@ -188,14 +230,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7])
       : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
-      " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -242,10 +276,10 @@ __device__ __forceinline__ uint32_t fp4_idesc(int nn) {
 
 // ---- work units -----------------------------------------------------------------
 
-template <class G, class S>
+template <class S>
 __device__ __forceinline__ int chunks_of(const S& s, int e) {
   const int n = s.offs[e + 1] - s.offs[e];
-  return n > 0 ? (n + G::kTok - 1) / G::kTok : 0;
+  return n > 0 ? (n + kTok - 1) / kTok : 0;
 }
 
 // n-tile n of expert e against `rows` tokens from row0 on.
@@ -256,7 +290,7 @@ struct Unit {
 // The largest e with cum[e] <= id is the (non-empty) expert that owns the
 // unit; its units are ordered (n-tile, chunk), the chunk fastest.  The chunks
 // are equal up to the rounding to 16 rows.
-template <class G, class S>
+template <class S>
 __device__ __forceinline__ Unit decode_unit(const S& s, int num_experts, int id) {
   int lo = 0, hi = num_experts - 1;
   while (lo < hi) {
@@ -267,7 +301,7 @@ __device__ __forceinline__ Unit decode_unit(const S& s, int num_experts, int id)
   Unit u;
   u.e = lo;
   const int local = id - s.cum[lo];
-  const int c = chunks_of<G>(s, lo);
+  const int c = chunks_of(s, lo);
   u.n = local / c;
   const int m = local - u.n * c;
   const int n = s.offs[lo + 1] - s.offs[lo];
@@ -279,17 +313,9 @@ __device__ __forceinline__ Unit decode_unit(const S& s, int num_experts, int id)
 
 template <bool SWIGLU, class G>
 __global__ void __launch_bounds__(kThreads, 1)
-    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a64,
-                    const __grid_constant__ CUtensorMap tmap_a16,
-                    const __grid_constant__ CUtensorMap tmap_b,
-                    const __grid_constant__ CUtensorMap tmap_s64,
-                    const __grid_constant__ CUtensorMap tmap_s16, const __grid_constant__ Params p) {
+    fp4_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using Smem = SmemT<G>;
-  constexpr int S = G::kStages;
-  constexpr int SS = G::kSfStages;
-  constexpr int kTokOff = 2 * kBoxBytes;
-  constexpr int kSfTokOff = 2 * kSfBoxBytes;            // token scales, 16 bytes a row
-  constexpr int kSfTokCols = 4 * G::kHalves;            // TMEM columns of the tokens' scales of an MMA
+  constexpr int kSfTokCols = 4 * kHalves;            // TMEM columns of the tokens' scales of an MMA
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                      ~static_cast<uintptr_t>(1023));
@@ -311,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int eb = min(E, tid * per);
     const int ee = min(E, eb + per);
     int local = 0;
-    for (int e = eb; e < ee; ++e) local += chunks_of<G>(s, e) * p.n_tiles;
+    for (int e = eb; e < ee; ++e) local += chunks_of(s, e) * p.n_tiles;
     int incl = local;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -324,17 +350,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int w = 0; w < warp; ++w) run += s.warp_tot[w];
     for (int e = eb; e < ee; ++e) {
       s.cum[e] = run;
-      run += chunks_of<G>(s, e) * p.n_tiles;
+      run += chunks_of(s, e) * p.n_tiles;
     }
     if (eb < E && ee == E) s.cum[E] = run;
   }
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < S; ++i) {
+    for (int i = 0; i < kRecs; ++i) {
       mbar_init(&s.full_bar[i], 2);  // both producers of codes
       mbar_init(&s.empty_bar[i], 1);
     }
-    for (int i = 0; i < SS; ++i) {
+    for (int i = 0; i < kSfStages; ++i) {
       mbar_init(&s.sf_full_bar[i], 1);
       mbar_init(&s.sf_empty_bar[i], kSfWarps);
     }
@@ -349,9 +375,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&s.q_empty[i], 1 + kEpiWarps + kSfWarps + 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a64)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_a16)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_b)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.b)) : "memory");
+    for (int i = 0; i < 4; ++i)
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.a[i])) : "memory");
+    for (int i = 0; i < 4 && p.sf_by_tma; ++i)
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.s[i])) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -373,17 +401,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto cols_of = [&](const Unit& u) { return min(p.out_tile_cols, p.n_out - u.n * p.out_tile_cols); };
   auto boxes_of = [&](const Unit& u) { return SWIGLU || cols_of(u) > kBoxRows ? 2 : 1; };
 
+  // Both producers of codes: waits until a stage of `span` bytes and its record
+  // are free; false on abort.  `held` and `j_free` count what this producer has
+  // not yet seen released.
+  auto reserve = [&](uint32_t* spans, uint32_t j, uint32_t span, uint32_t& j_free,
+                     uint32_t& held) -> bool {
+    while (j - j_free >= static_cast<uint32_t>(kRecs) || held + span > G::kRing) {
+      const uint32_t r = j_free % kRecs;
+      if (!wait_bar(&s.empty_bar[r], (j_free / kRecs) & 1u, abort, kDevErrGemmProducerWait)) return false;
+      held -= spans[r];
+      ++j_free;
+    }
+    spans[j % kRecs] = span;
+    held += span;
+    return true;
+  };
+  // Token rows r, r + 16 << i, ... of a unit in the largest boxes that fit.
+  auto box_of = [](int left) { return left >= 128 ? 3 : left >= 64 ? 2 : left >= 32 ? 1 : 0; };
+
   if (warp == 0) {
     // ===================== units; TMA producer of the weights' codes =====================
     if (elect_one()) {
       // Normal eviction: the other chunks of an expert find the weights in L2.
       const uint64_t policy = policy_evict_normal();
       bool ok = true;
-      uint32_t j = 0;  // stages issued so far
+      RingPos<G> pos;
+      uint32_t j_free = 0, held = 0;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
-        if (!wait_bar(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort,
-                       kDevErrGemmProducerWait)) {
+        if (!wait_bar(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort, kDevErrGemmProducerWait)) {
           ok = false;
           break;
         }
@@ -393,25 +439,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         s.unit_q[qslot] = unit;
         mbar_arrive(&s.q_full[qslot]);
         if (unit < 0) break;
-        const Unit u = decode_unit<G>(s, E, unit);
+        const Unit u = decode_unit(s, E, unit);
         const int boxes = boxes_of(u);
+        const uint32_t tok_bytes = ((u.rows + 15) & ~15) * kRowBytes;
         const int brow = u.e * p.b_rows + u.n * p.b_tile_rows;
-        for (int kb = 0; kb < num_kb; ++kb, ++j) {
-          const uint32_t slot = j % S;
-          if (!wait_bar(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait)) {
+        for (int kb = 0; kb < num_kb; ++kb, ++pos.j) {
+          const uint32_t span = pos.layout(boxes, tok_bytes);
+          if (!reserve(s.span[0], pos.j, span, j_free, held)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&s.full_bar[slot], boxes * kBoxBytes);
-          tma_load_2d(s.ring[slot], &tmap_b, &s.full_bar[slot], kb * kRowBytes, brow, policy);
+          uint64_t* full = &s.full_bar[pos.rec()];
+          mbar_expect_tx(full, boxes * kBoxBytes);
+          tma_load_2d(s.ring + pos.w0, &maps.b, full, kb * kRowBytes, brow, policy);
           if (boxes == 2)
-            tma_load_2d(s.ring[slot] + kBoxBytes, &tmap_b, &s.full_bar[slot], kb * kRowBytes,
-                        brow + p.b_second, policy);
+            tma_load_2d(s.ring + pos.w1, &maps.b, full, kb * kRowBytes, brow + p.b_second, policy);
         }
       }
       if (!ok) {  // let every issued load land before the CTA can exit
-        for (uint32_t d = j > S ? j - S : 0; d < j; ++d)
-          mbar_wait(&s.full_bar[d % S], (d / S) & 1u, abort, kDevErrGemmProducerWait, false);
+        for (uint32_t d = j_free; d < pos.j; ++d)
+          mbar_wait(&s.full_bar[d % kRecs], (d / kRecs) & 1u, abort, kDevErrGemmProducerWait, false);
       }
     }
   } else if (warp == kTokWarp) {
@@ -419,7 +466,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect_one()) {
       const uint64_t policy = policy_evict_last();  // read by every n-tile
       bool ok = true;
-      uint32_t j = 0;
+      RingPos<G> pos;
+      uint32_t j_free = 0, held = 0;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
         if (!wait_bar(&s.q_full[qslot], (qn / kUnitQ) & 1u, abort, kDevErrGemmProducerWait)) {
@@ -429,31 +477,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int unit = s.unit_q[qslot];
         mbar_arrive(&s.q_empty[qslot]);
         if (unit < 0) break;
-        const Unit u = decode_unit<G>(s, E, unit);
+        const Unit u = decode_unit(s, E, unit);
         const int nn = (u.rows + 15) & ~15;
-        for (int kb = 0; kb < num_kb; ++kb, ++j) {
-          const uint32_t slot = j % S;
-          if (!wait_bar(&s.empty_bar[slot], ((j / S) & 1u) ^ 1u, abort, kDevErrGemmProducerWait)) {
+        const int boxes = boxes_of(u);
+        for (int kb = 0; kb < num_kb; ++kb, ++pos.j) {
+          const uint32_t span = pos.layout(boxes, nn * kRowBytes);
+          if (!reserve(s.span[1], pos.j, span, j_free, held)) {
             ok = false;
             break;
           }
-          mbar_expect_tx(&s.full_bar[slot], nn * kRowBytes);
+          uint64_t* full = &s.full_bar[pos.rec()];
+          mbar_expect_tx(full, nn * kRowBytes);
           for (int r = 0; r < nn;) {
-            const bool big = r + 64 <= nn;
-            tma_load_2d(s.ring[slot] + kTokOff + r * kRowBytes, big ? &tmap_a64 : &tmap_a16,
-                        &s.full_bar[slot], kb * kRowBytes, u.row0 + r, policy);
-            r += big ? 64 : 16;
+            const int i = box_of(nn - r);
+            tma_load_2d(s.ring + pos.tok + r * kRowBytes, &maps.a[i], full, kb * kRowBytes,
+                        u.row0 + r, policy);
+            r += 16 << i;
           }
         }
       }
       if (!ok) {
-        for (uint32_t d = j > S ? j - S : 0; d < j; ++d)
-          mbar_wait(&s.full_bar[d % S], (d / S) & 1u, abort, kDevErrGemmProducerWait, false);
+        for (uint32_t d = j_free; d < pos.j; ++d)
+          mbar_wait(&s.full_bar[d % kRecs], (d / kRecs) & 1u, abort, kDevErrGemmProducerWait, false);
       }
     }
   } else if (warp == kSfLoadWarp) {
     // ===================== TMA producer of scales =====================
-    // Runs up to SS stages ahead of the scale warps, which release a slot as
+    // Runs up to kSfStages stages ahead of the scale warps, which release a slot as
     // soon as they have read it, so scales wait in TMEM before their codes land.
     if (elect_one()) {
       const uint64_t policy = policy_evict_last();
@@ -468,15 +518,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int unit = s.unit_q[qslot];
         mbar_arrive(&s.q_empty[qslot]);
         if (unit < 0) break;
-        const Unit u = decode_unit<G>(s, E, unit);
+        const Unit u = decode_unit(s, E, unit);
         const int nn = (u.rows + 15) & ~15;
         const int boxes = boxes_of(u);
         const uint8_t* sf = p.b_sf + static_cast<int64_t>(u.e * p.sf_tiles + u.n * p.sf_tile_step) *
                                          p.steps * kSfTile;
         const uint8_t* sf2 = sf + static_cast<int64_t>(p.sf_second) * p.steps * kSfTile;
         for (int kb = 0; kb < num_kb; ++kb, ++j) {
-          const uint32_t slot = j % SS;
-          if (!wait_bar(&s.sf_empty_bar[slot], ((j / SS) & 1u) ^ 1u, abort, kDevErrGemmScaleWait)) {
+          const uint32_t slot = j % kSfStages;
+          if (!wait_bar(&s.sf_empty_bar[slot], ((j / kSfStages) & 1u) ^ 1u, abort, kDevErrGemmScaleWait)) {
             ok = false;
             break;
           }
@@ -488,24 +538,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (boxes == 2) bulk_load(st + kSfBoxBytes, sf2 + kb * kSfBoxBytes, bytes, full);
           if (p.sf_by_tma) {
             for (int r = 0; r < nn;) {
-              const bool big = r + 64 <= nn;
-              tma_load_2d(st + kSfTokOff + r * 16, big ? &tmap_s64 : &tmap_s16, full, kb * 16,
-                          u.row0 + r, policy);
-              r += big ? 64 : 16;
+              const int i = box_of(nn - r);
+              tma_load_2d(st + kSfTokOff + r * 16, &maps.s[i], full, kb * 16, u.row0 + r, policy);
+              r += 16 << i;
             }
           }
         }
       }
       if (!ok) {
-        for (uint32_t d = j > SS ? j - SS : 0; d < j; ++d)
-          mbar_wait(&s.sf_full_bar[d % SS], (d / SS) & 1u, abort, kDevErrGemmScaleWait, false);
+        for (uint32_t d = j > kSfStages ? j - kSfStages : 0; d < j; ++d)
+          mbar_wait(&s.sf_full_bar[d % kSfStages], (d / kSfStages) & 1u, abort, kDevErrGemmScaleWait, false);
       }
     }
   } else if (warp == 1) {
     // ===================== MMA issuer =====================
     if (elect_one()) {
       uint32_t ac = 0;  // accumulator slots taken so far
-      uint32_t j = 0;   // stages consumed so far
+      RingPos<G> pos;
+      const uint32_t ring = smem_u32(s.ring);
       bool ok = true;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
@@ -513,15 +563,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int unit = s.unit_q[qslot];
         mbar_arrive(&s.q_empty[qslot]);
         if (unit < 0) break;
-        const Unit u = decode_unit<G>(s, E, unit);
+        const Unit u = decode_unit(s, E, unit);
         const int nn = (u.rows + 15) & ~15;
         const int boxes = boxes_of(u);
         const uint32_t idesc = fp4_idesc(nn);
         const bool two = nn > kAccCols / 2;  // the unit takes both slots
         const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
         if (!wait_bar(&s.acc_empty_bar[acc0], ((ac >> 1) & 1u) ^ 1u, abort, kDevErrGemmMmaWait) ||
-            (two && !mbar_wait(&s.acc_empty_bar[acc1], (((ac + 1) >> 1) & 1u) ^ 1u, abort,
-                               kDevErrGemmMmaWait, true))) {
+            (two && !wait_bar(&s.acc_empty_bar[acc1], (((ac + 1) >> 1) & 1u) ^ 1u, abort,
+                              kDevErrGemmMmaWait))) {
           ok = false;
           break;
         }
@@ -529,28 +579,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d0 = tmem_base + (two ? 0u : acc0 * kAccCols);
         const uint32_t d1 = d0 + (two ? kAccCols : kAccCols / 2);
-        for (int kb = 0; kb < num_kb; ++kb, ++j) {
-          const int slot = j % S;
-          if (!wait_bar(&s.full_bar[slot], (j / S) & 1u, abort, kDevErrGemmMmaWait) ||
+        for (int kb = 0; kb < num_kb; ++kb, ++pos.j) {
+          const int rec = pos.rec();
+          const uint32_t j = pos.j;
+          pos.layout(boxes, nn * kRowBytes);
+          if (!wait_bar(&s.full_bar[rec], pos.parity(), abort, kDevErrGemmMmaWait) ||
               !wait_bar(&s.sf_bar[j & 1u], (j >> 1) & 1u, abort, kDevErrGemmMmaWait)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t st = smem_u32(s.ring[slot]);
           const uint32_t sfb = tmem_base + kSfCol + (j & 1u) * kSfBufCols;  // weights
           const uint32_t sft = sfb + 2 * kSteps * 4;                        // tokens
           const int steps = min(kSteps, p.steps - kb * kSteps);
           for (int k = 0; k < steps; ++k) {
-            const uint64_t tok = smem_desc_sw128(st + kTokOff + k * 32);
+            const uint64_t tok = smem_desc_sw128(ring + pos.tok + k * 32);
             const uint32_t acc_in = (kb | k) != 0 ? 1u : 0u;
-            umma_fp4(d0, smem_desc_sw128(st + k * 32), tok, idesc, sfb + k * 8,
+            umma_fp4(d0, smem_desc_sw128(ring + pos.w0 + k * 32), tok, idesc, sfb + k * 8,
                      sft + k * kSfTokCols, acc_in);
             if (boxes == 2)
-              umma_fp4(d1, smem_desc_sw128(st + kBoxBytes + k * 32), tok, idesc, sfb + k * 8 + 4,
+              umma_fp4(d1, smem_desc_sw128(ring + pos.w1 + k * 32), tok, idesc, sfb + k * 8 + 4,
                        sft + k * kSfTokCols, acc_in);
           }
-          umma_commit(&s.empty_bar[slot]);
+          umma_commit(&s.empty_bar[rec]);
         }
         if (ok) {
           umma_commit(&s.acc_full_bar[acc0]);
@@ -576,12 +627,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.q_empty[qslot]);
       if (unit < 0) break;
-      const Unit u = decode_unit<G>(s, E, unit);
+      const Unit u = decode_unit(s, E, unit);
       // Without TMA: the scales of stage kb of token row 32 q + lane, word k
       // for MMA k.  Rows past the unit and MMAs past K get zeros.
-      auto load_tok = [&](int kb, uint32_t (&t)[4 * G::kHalves][kSteps]) {
+      auto load_tok = [&](int kb, uint32_t (&t)[4 * kHalves][kSteps]) {
 #pragma unroll
-        for (int q = 0; q < 4 * G::kHalves; ++q) {
+        for (int q = 0; q < 4 * kHalves; ++q) {
           const int r = q * 32 + lane;
           const uint8_t* src = p.a_sf + static_cast<int64_t>(u.row0 + r) * sf_row + kb * (4 * kSteps);
 #pragma unroll
@@ -591,11 +642,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                           : 0u;
         }
       };
-      uint32_t tok[4 * G::kHalves][kSteps];
+      uint32_t tok[4 * kHalves][kSteps];
       for (int kb = 0; kb < num_kb; ++kb, ++j) {
-        const uint32_t slot = j % SS;
+        const uint32_t slot = j % kSfStages;
         if (!p.sf_by_tma) load_tok(kb, tok);
-        ok = __all_sync(0xffffffffu, wait_bar(&s.sf_full_bar[slot], (j / SS) & 1u, abort,
+        ok = __all_sync(0xffffffffu, wait_bar(&s.sf_full_bar[slot], (j / kSfStages) & 1u, abort,
                                                kDevErrGemmScaleWait));
         if (!ok) break;
         const uint8_t* image = s.sf_ring[slot] + lane * 16;
@@ -612,8 +663,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         if (p.sf_by_tma) {
 #pragma unroll
-          for (int q = 0; q < 4 * G::kHalves; ++q)
-            if (q * 32 < G::kTok) {
+          for (int q = 0; q < 4 * kHalves; ++q)
+            if (q * 32 < kTok) {
               const uint4 v = *reinterpret_cast<const uint4*>(image + kSfTokOff + q * 512);
               tok[q][0] = v.x;
               tok[q][1] = v.y;
@@ -625,22 +676,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-          for (int q = 0; q < 4 * G::kHalves; ++q)
-            t[k * kSfTokCols + q] = q * 32 < G::kTok ? tok[q][k] : 0u;
+          for (int q = 0; q < 4 * kHalves; ++q)
+            t[k * kSfTokCols + q] = q * 32 < kTok ? tok[q][k] : 0u;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.sf_empty_bar[slot]);
         // The MMAs of two stages before, which read this buffer, have completed.
         if (j >= 2)
-          ok = __all_sync(0xffffffffu, wait_bar(&s.empty_bar[(j - 2) % S], ((j - 2) / S) & 1u,
+          ok = __all_sync(0xffffffffu, wait_bar(&s.empty_bar[(j - 2) % kRecs], ((j - 2) / kRecs) & 1u,
                                                  abort, kDevErrGemmScaleWait));
         if (!ok) break;
         tc_fence_after();
         const uint32_t col = tmem_base + quarter + kSfCol + (j & 1u) * kSfBufCols;
         tmem_st32(col, w);
-        if constexpr (G::kHalves == 2)
-          tmem_st32(col + 2 * kSteps * 4, t);
-        else
-          tmem_st16(col + 2 * kSteps * 4, t);
+        tmem_st32(col + 2 * kSteps * 4, t);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -665,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.q_empty[qslot]);
       if (unit < 0) break;
-      const Unit u = decode_unit<G>(s, E, unit);
+      const Unit u = decode_unit(s, E, unit);
       const int nn = (u.rows + 15) & ~15;
       const bool two = nn > kAccCols / 2;
       const uint32_t acc0 = ac & 1u, acc1 = (ac + 1) & 1u;
@@ -685,9 +733,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int feat = q * 32 + (lane & 1) * 16;  // first of 16 output columns of the box
       const uint4* mine = reinterpret_cast<const uint4*>(turn + tok * kStagePitch + (lane & 1) * 32);
       // Drain: both boxes as a bf16 pair for each token of this warp's chunks.
-      uint32_t pair[G::kChunks][16];
+      uint32_t pair[kChunks][16];
 #pragma unroll
-      for (int c = 0; c < G::kChunks; ++c) {
+      for (int c = 0; c < kChunks; ++c) {
         const int t0 = (2 * c + grp) * 16;
         if (t0 < nn) {
 #pragma unroll
@@ -710,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
       }
 #pragma unroll
-      for (int c = 0; c < G::kChunks; ++c) {
+      for (int c = 0; c < kChunks; ++c) {
         const int t0 = (2 * c + grp) * 16;
         if (t0 >= nn) break;
         const int64_t row = u.row0 + t0 + tok;
@@ -793,25 +841,22 @@ lsek_status launch_geom(Params p, const void* A, const void* B, int K, cudaStrea
                                 static_cast<int>(smem_bytes<G>()));
   });
   if (ae != cudaSuccess) return fail(LSEK_ERR_CUDA, "grouped_gemm_nvfp4: %s", cudaGetErrorString(ae));
-  CUtensorMap a64, a16, b, s64, s16;
+  Maps m{};
   const uint64_t row_bytes = static_cast<uint64_t>(K) / 2;
-  lsek_status s = make_map(&a64, A, row_bytes, static_cast<uint64_t>(p.rows), 64u);
-  if (s == LSEK_OK) s = make_map(&a16, A, row_bytes, static_cast<uint64_t>(p.rows), 16u);
-  if (s == LSEK_OK)
-    s = make_map(&b, B, row_bytes, static_cast<uint64_t>(p.num_experts) * p.b_rows,
-                 static_cast<uint32_t>(kBoxRows));
-  s64 = s16 = a16;  // unused without TMA
-  if (s == LSEK_OK && p.sf_by_tma) {
-    s = make_map(&s64, p.a_sf, row_bytes / 8, static_cast<uint64_t>(p.rows), 64u, 16u);
-    if (s == LSEK_OK) s = make_map(&s16, p.a_sf, row_bytes / 8, static_cast<uint64_t>(p.rows), 16u, 16u);
+  lsek_status s = make_map(&m.b, B, row_bytes, static_cast<uint64_t>(p.num_experts) * p.b_rows,
+                           static_cast<uint32_t>(kBoxRows));
+  for (int i = 0; i < 4 && s == LSEK_OK; ++i) {
+    s = make_map(&m.a[i], A, row_bytes, static_cast<uint64_t>(p.rows), 16u << i);
+    if (s == LSEK_OK && p.sf_by_tma)
+      s = make_map(&m.s[i], p.a_sf, row_bytes / 8, static_cast<uint64_t>(p.rows), 16u << i, 16u);
   }
   if (s != LSEK_OK) return s;
   if (p.counter != nullptr) LSEK_CUDA_TRY(cudaMemsetAsync(p.counter, 0, sizeof(int32_t), st));
   // At most rows / kTok full chunks and one partial chunk per non-empty expert.
   const int64_t experts = p.num_experts < p.rows ? p.num_experts : p.rows;
-  const int64_t max_units = (p.rows / G::kTok + experts) * static_cast<int64_t>(p.n_tiles);
+  const int64_t max_units = (p.rows / kTok + experts) * static_cast<int64_t>(p.n_tiles);
   const int grid = static_cast<int>(max_units < num_sms() ? max_units : num_sms());
-  fp4_gemm_kernel<SWIGLU, G><<<grid, kThreads, smem_bytes<G>(), st>>>(a64, a16, b, s64, s16, p);
+  fp4_gemm_kernel<SWIGLU, G><<<grid, kThreads, smem_bytes<G>(), st>>>(m, p);
   return check_launch(SWIGLU ? "grouped_gemm_swiglu_nvfp4" : "grouped_gemm_nvfp4");
 }
 
@@ -825,14 +870,12 @@ lsek_status fp4_take_device_error(int32_t* code) {
 }
 
 // Both products; D for the plain one, h_codes / h_scales for gate/up + SwiGLU
-// (n_out = I there).  max_rows_per_expert: an upper bound, or -1; every
-// argument has been checked.
+// (n_out = I there).  Every argument has been checked.
 lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales, const void* A,
                              const void* a_scales, const void* B, const void* b_tiles,
                              const int32_t* offsets, const float* a_global, const float* b_global,
                              const float* out_global, int E, int rows, int n_out, int K,
-                             float limit, int32_t* counter, cudaStream_t st,
-                             int max_rows_per_expert) {
+                             float limit, int32_t* counter, cudaStream_t st) {
   using namespace fp4;
   if (rows == 0 || n_out == 0) return LSEK_OK;
   Params p{};
@@ -871,12 +914,11 @@ lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales
     p.out_tile_cols = 2 * kBoxRows;
   }
   p.n_tiles = static_cast<int>(ceil_div(n_out, p.out_tile_cols));
-  const int bound = max_rows_per_expert >= 0 && max_rows_per_expert < rows ? max_rows_per_expert : rows;
-  if (bound <= GeomDecode::kTok)
-    return swiglu ? launch_geom<true, GeomDecode>(p, A, B, K, st)
-                  : launch_geom<false, GeomDecode>(p, A, B, K, st);
-  return swiglu ? launch_geom<true, GeomFull>(p, A, B, K, st)
-                : launch_geom<false, GeomFull>(p, A, B, K, st);
+  if (E <= GeomFull::kMaxE)
+    return swiglu ? launch_geom<true, GeomFull>(p, A, B, K, st)
+                  : launch_geom<false, GeomFull>(p, A, B, K, st);
+  return swiglu ? launch_geom<true, GeomWide>(p, A, B, K, st)
+                : launch_geom<false, GeomWide>(p, A, B, K, st);
 }
 
 namespace {
@@ -924,7 +966,7 @@ extern "C" lsek_status lsek_grouped_gemm_nvfp4(void* D, const void* A, const voi
   if (s != LSEK_OK) return s;
   return grouped_gemm_fp4(false, D, nullptr, nullptr, A, a_scales, B, b_scale_tiles, expert_offsets,
                           a_global_scale, b_global_scale, nullptr, num_experts, rows, N, K, 0.0f,
-                          counter_in(workspace, workspace_bytes), static_cast<cudaStream_t>(stream), -1);
+                          counter_in(workspace, workspace_bytes), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" lsek_status lsek_grouped_gemm_swiglu_nvfp4(
@@ -943,5 +985,5 @@ extern "C" lsek_status lsek_grouped_gemm_swiglu_nvfp4(
   return grouped_gemm_fp4(true, nullptr, h_codes, h_scales, A, a_scales, W_gu, gu_scale_tiles,
                           expert_offsets, a_global_scale, gu_global_scale, h_global_scale,
                           num_experts, rows, I, K, swiglu_limit, counter_in(workspace, workspace_bytes),
-                          static_cast<cudaStream_t>(stream), -1);
+                          static_cast<cudaStream_t>(stream));
 }
