@@ -3,7 +3,7 @@
 // All three are HBM streams: the quantiser reads 2 bytes and writes 0.5625
 // bytes an element, the dequantiser the reverse, and the permute reads each
 // token once and writes 0.5625 bytes an element to each of its topk rows.
-// One thread takes one block of 16 elements: 32 bytes in (two 16-byte loads),
+// One thread takes a block of 16 elements at a time: 32 bytes in (one access),
 // 8 bytes of codes and one scale byte out, so a warp reads 1 KB and writes
 // 256 + 32 bytes, all contiguous.  Blocks do not cross rows (the row length is
 // a multiple of 16), so a contiguous tensor is one flat run of blocks.
@@ -17,13 +17,27 @@ lsek_status launch_route_by_expert(const int32_t* idx, int64_t n, int E, int32_t
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnroll = 4;                            // blocks a thread has in flight
+constexpr int kCtaBlocks = kThreads * kUnroll;
 
-// One block of 16 elements; VEC: the address is a multiple of 16 bytes.
+// 32 bytes in one access (the address a multiple of 32).
+__device__ __forceinline__ void ldg_nc_v8(const void* p, uint4& lo, uint4& hi) {
+  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y),
+                 "=r"(hi.z), "=r"(hi.w)
+               : "l"(p));
+}
+__device__ __forceinline__ void stg_v8(void* p, const uint4& lo, const uint4& hi) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(lo.x), "r"(lo.y),
+               "r"(lo.z), "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
+               : "memory");
+}
+
+// One block of 16 elements; VEC: the address is a multiple of 32 bytes.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_block(const T* p, uint4& lo, uint4& hi) {
   if (VEC) {
-    lo = ldg_nc_v4(p);
-    hi = ldg_nc_v4(p + 8);
+    ldg_nc_v8(p, lo, hi);
   } else {
     uint16_t v[16];
 #pragma unroll
@@ -35,32 +49,48 @@ __device__ __forceinline__ void load_block(const T* p, uint4& lo, uint4& hi) {
 }
 
 // `blocks` blocks in groups of `group_blocks`, one global scale per group
-// (global == null: 1).
+// (global == null: 1).  A thread takes kUnroll blocks kThreads apart and loads
+// them all before it works on the first.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(uint2* __restrict__ codes, uint8_t* __restrict__ scales,
                     const T* __restrict__ x, const float* __restrict__ global, int64_t blocks,
                     int64_t group_blocks) {
-  const int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
-  if (i >= blocks) return;
-  const float g = global ? __ldg(global + i / group_blocks) : 1.0f;
-  uint4 lo, hi;
-  load_block<T, VEC>(x + i * kFp4Block, lo, hi);
-  const Fp4Block q = fp4_quantize16<T>(lo, hi, g, __fmul_rn(6.0f, g));
-  codes[i] = q.codes;
-  scales[i] = static_cast<uint8_t>(q.scale);
+  const int64_t first = blockIdx.x * static_cast<int64_t>(kCtaBlocks) + threadIdx.x;
+  uint4 lo[kUnroll], hi[kUnroll];
+  float g[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = first + u * kThreads;
+    if (i >= blocks) break;
+    load_block<T, VEC>(x + i * kFp4Block, lo[u], hi[u]);
+    g[u] = global ? __ldg(global + i / group_blocks) : 1.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = first + u * kThreads;
+    if (i >= blocks) break;
+    const Fp4Block q = fp4_quantize16<T>(lo[u], hi[u], g[u], __fmul_rn(6.0f, g[u]));
+    codes[i] = q.codes;
+    scales[i] = static_cast<uint8_t>(q.scale);
+  }
 }
 
-template <typename T>
+template <typename T, bool VEC>
 __device__ __forceinline__ void store_block(T* p, const float (&v)[16]) {
   Vec8<T> o[2];
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i / 8].v[i % 8] = Elem<T>::from_f(v[i]);
-  reinterpret_cast<uint4*>(p)[0] = *reinterpret_cast<const uint4*>(&o[0]);
-  reinterpret_cast<uint4*>(p)[1] = *reinterpret_cast<const uint4*>(&o[1]);
+  const uint4 lo = *reinterpret_cast<const uint4*>(&o[0]), hi = *reinterpret_cast<const uint4*>(&o[1]);
+  if (VEC) {
+    stg_v8(p, lo, hi);
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = lo;
+    reinterpret_cast<uint4*>(p)[1] = hi;
+  }
 }
 template <>
-__device__ __forceinline__ void store_block<float>(float* p, const float (&v)[16]) {
+__device__ __forceinline__ void store_block<float, false>(float* p, const float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -68,24 +98,37 @@ __device__ __forceinline__ void store_block<float>(float* p, const float (&v)[16
 
 // code * scale is exact in fp32 (2 + 4 significand bits); the product with g
 // is rounded once, and once more to a 16-bit output type.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     dequantize_kernel(T* __restrict__ out, const uint2* __restrict__ codes,
                       const uint8_t* __restrict__ scales, const float* __restrict__ global,
                       int64_t blocks, int64_t group_blocks) {
-  const int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x;
-  if (i >= blocks) return;
-  const float g = global ? __ldg(global + i / group_blocks) : 1.0f;
-  const uint2 c = __ldg(codes + i);
-  const float s = e4m3_to_f32(__ldg(scales + i));
-  float v[16];
+  const int64_t first = blockIdx.x * static_cast<int64_t>(kCtaBlocks) + threadIdx.x;
+  uint2 c[kUnroll];
+  uint32_t sc[kUnroll];
+  float g[kUnroll];
 #pragma unroll
-  for (int b = 0; b < 8; ++b) {
-    const float2 two = e2m1x2_to_f32((b < 4 ? c.x : c.y) >> (8 * (b & 3)) & 0xFFu);
-    v[2 * b] = __fmul_rn(__fmul_rn(two.x, s), g);
-    v[2 * b + 1] = __fmul_rn(__fmul_rn(two.y, s), g);
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = first + u * kThreads;
+    if (i >= blocks) break;
+    c[u] = __ldg(codes + i);
+    sc[u] = __ldg(scales + i);
+    g[u] = global ? __ldg(global + i / group_blocks) : 1.0f;
   }
-  store_block<T>(out + i * kFp4Block, v);
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t i = first + u * kThreads;
+    if (i >= blocks) break;
+    const float s = e4m3_to_f32(sc[u]);
+    float v[16];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const float2 two = e2m1x2_to_f32((b < 4 ? c[u].x : c[u].y) >> (8 * (b & 3)) & 0xFFu);
+      v[2 * b] = __fmul_rn(__fmul_rn(two.x, s), g[u]);
+      v[2 * b + 1] = __fmul_rn(__fmul_rn(two.y, s), g[u]);
+    }
+    store_block<T, VEC>(out + i * kFp4Block, v);
+  }
 }
 
 // Quantises each token once and stores it to its topk rows.  Grid (T, slices
@@ -116,7 +159,6 @@ lsek_status check_blocks(const char* name, int64_t groups, int64_t rows, int32_t
   LSEK_REQUIRE(groups >= 0 && rows >= 0 && k >= 0, "%s: sizes must be >= 0", name);
   LSEK_REQUIRE(k % kFp4Block == 0, "%s: the row length must be a multiple of %d, got %d", name,
                kFp4Block, k);
-  // grid.x holds the blocks in units of kThreads
   LSEK_REQUIRE(groups == 0 || rows <= (1ll << 38) / groups, "%s: too many rows", name);
   LSEK_REQUIRE(k == 0 || groups * rows <= (1ll << 38) / (k / kFp4Block),
                "%s: more than 2^38 blocks of %d", name, kFp4Block);
@@ -126,11 +168,11 @@ lsek_status check_blocks(const char* name, int64_t groups, int64_t rows, int32_t
 template <typename T>
 lsek_status quantize_t(void* codes, void* scales, const void* x, const float* global,
                        int64_t blocks, int64_t group_blocks, cudaStream_t st) {
-  const unsigned grid = static_cast<unsigned>(ceil_div(blocks, kThreads));
+  const unsigned grid = static_cast<unsigned>(ceil_div(blocks, kCtaBlocks));
   uint2* c = static_cast<uint2*>(codes);
   uint8_t* s = static_cast<uint8_t*>(scales);
   const T* in = static_cast<const T*>(x);
-  if (aligned(x, 16))
+  if (aligned(x, 32))
     quantize_kernel<T, true><<<grid, kThreads, 0, st>>>(c, s, in, global, blocks, group_blocks);
   else
     quantize_kernel<T, false><<<grid, kThreads, 0, st>>>(c, s, in, global, blocks, group_blocks);
@@ -150,7 +192,7 @@ lsek_status launch_permute_quantize(void* codes, void* scales, const void* hidde
   uint2* c = static_cast<uint2*>(codes);
   uint8_t* s = static_cast<uint8_t*>(scales);
   const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(hidden);
-  if (aligned(hidden, 16))
+  if (aligned(hidden, 32))
     permute_quantize_kernel<true><<<grid, kThreads, 0, st>>>(c, s, in, s2d, global, topk, row_blocks);
   else
     permute_quantize_kernel<false><<<grid, kThreads, 0, st>>>(c, s, in, s2d, global, topk, row_blocks);
@@ -190,18 +232,20 @@ extern "C" lsek_status lsek_nvfp4_dequantize(void* out, const void* codes, const
   LSEK_REQUIRE(aligned(codes, 8) && aligned(out, 16),
                "nvfp4_dequantize: codes must be 8-byte aligned, out 16-byte");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(ceil_div(blocks, kThreads));
+  const unsigned grid = static_cast<unsigned>(ceil_div(blocks, kCtaBlocks));
   const uint2* c = static_cast<const uint2*>(codes);
   const uint8_t* sc = static_cast<const uint8_t*>(scales);
+  const bool vec = aligned(out, 32);
+  auto run = [&](auto* o, auto kernel, auto kernel_vec) {
+    (vec ? kernel_vec : kernel)<<<grid, kThreads, 0, st>>>(o, c, sc, global_scale, blocks, group_blocks);
+  };
   if (dtype == LSEK_BF16)
-    dequantize_kernel<<<grid, kThreads, 0, st>>>(static_cast<__nv_bfloat16*>(out), c, sc,
-                                                 global_scale, blocks, group_blocks);
+    run(static_cast<__nv_bfloat16*>(out), dequantize_kernel<__nv_bfloat16, false>,
+        dequantize_kernel<__nv_bfloat16, true>);
   else if (dtype == LSEK_FP16)
-    dequantize_kernel<<<grid, kThreads, 0, st>>>(static_cast<__half*>(out), c, sc, global_scale,
-                                                 blocks, group_blocks);
+    run(static_cast<__half*>(out), dequantize_kernel<__half, false>, dequantize_kernel<__half, true>);
   else
-    dequantize_kernel<<<grid, kThreads, 0, st>>>(static_cast<float*>(out), c, sc, global_scale,
-                                                 blocks, group_blocks);
+    run(static_cast<float*>(out), dequantize_kernel<float, false>, dequantize_kernel<float, false>);
   return check_launch("nvfp4_dequantize");
 }
 
