@@ -36,12 +36,12 @@ lsek_status grouped_gemm_swiglu_gather(void* H, const void* hidden, const void* 
 
 lsek_status launch_permute_quantize(void* codes, void* scales, const void* hidden,
                                     const int32_t* s2d, const float* global, int T, int topk,
-                                    int H, cudaStream_t st);
+                                    int H, int32_t* zero, int zeros, cudaStream_t st);
 lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales, const void* A,
                              const void* a_scales, const void* B, const void* b_tiles,
                              const int32_t* offsets, const float* a_global, const float* b_global,
                              const float* out_global, int E, int rows, int n_out, int K,
-                             float limit, int32_t* counter, cudaStream_t st);
+                             float limit, int32_t* counter, bool zero_counter, cudaStream_t st);
 
 namespace {
 struct LayerWs {
@@ -191,7 +191,8 @@ extern "C" size_t lsek_moe_layer_nvfp4_workspace_size(int32_t num_tokens, int32_
   return lsek::layer_fp4_ws(num_tokens, hidden_dim, inter_dim, num_experts, topk).total;
 }
 
-// The same flow on NVFP4 experts.  The tokens are quantised in the row copy,
+// The same flow on NVFP4 experts.  The row copy also zeroes the GEMMs' unit
+// counters (one each), which saves their memsets.  The tokens are quantised in the row copy,
 // so a slot's row is 0.5625 bytes an element, and h between the GEMMs exists
 // only in NVFP4 (the gate/up GEMM's epilogue quantises it).
 extern "C" lsek_status lsek_moe_layer_forward_nvfp4(
@@ -252,17 +253,17 @@ extern "C" lsek_status lsek_moe_layer_forward_nvfp4(
   if ((s = launch_route_by_expert(idx, n, E, offs, s2d, perm, st)) != LSEK_OK) return s;
   if ((s = mark(2)) != LSEK_OK) return s;
   s = launch_permute_quantize(ws + l.x, ws + l.xs, hidden, s2d, hidden_global_scale, T, k,
-                              hidden_dim, st);
+                              hidden_dim, counter, 2, st);
   if (s != LSEK_OK) return s;
   if ((s = mark(3)) != LSEK_OK) return s;
   s = grouped_gemm_fp4(true, nullptr, ws + l.h, ws + l.hs, ws + l.x, ws + l.xs, W_gu,
                        gu_scale_tiles, offs, hidden_global_scale, gu_global_scale,
-                       inter_global_scale, E, rows, inter_dim, hidden_dim, swiglu_limit, counter, st);
+                       inter_global_scale, E, rows, inter_dim, hidden_dim, swiglu_limit, counter, false, st);
   if (s != LSEK_OK) return s;
   if ((s = mark(4)) != LSEK_OK) return s;
   s = grouped_gemm_fp4(false, ws + l.y, nullptr, nullptr, ws + l.h, ws + l.hs, W_down,
                        down_scale_tiles, offs, inter_global_scale, down_global_scale, nullptr, E,
-                       rows, hidden_dim, inter_dim, 0.0f, counter, st);
+                       rows, hidden_dim, inter_dim, 0.0f, counter + 1, false, st);
   if (s != LSEK_OK) return s;
   if ((s = mark(5)) != LSEK_OK) return s;
   s = lsek_moe_unpermute(out, ws + l.y, w, s2d, T, k, hidden_dim, LSEK_BF16, 0, stream);

@@ -20,19 +20,6 @@ constexpr int kThreads = 256;
 constexpr int kUnroll = 4;                            // blocks a thread has in flight
 constexpr int kCtaBlocks = kThreads * kUnroll;
 
-// 32 bytes in one access (the address a multiple of 32).
-__device__ __forceinline__ void ldg_nc_v8(const void* p, uint4& lo, uint4& hi) {
-  asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y),
-                 "=r"(hi.z), "=r"(hi.w)
-               : "l"(p));
-}
-__device__ __forceinline__ void stg_v8(void* p, const uint4& lo, const uint4& hi) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(lo.x), "r"(lo.y),
-               "r"(lo.z), "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
-               : "memory");
-}
-
 // One block of 16 elements; VEC: the address is a multiple of 32 bytes.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_block(const T* p, uint4& lo, uint4& hi) {
@@ -132,14 +119,17 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Quantises each token once and stores it to its topk rows.  Grid (T, slices
-// of the row); a slice is kThreads blocks.
+// of the row); a slice is kThreads blocks.  `zero`: `zeros` words that the
+// caller wants zeroed on the way, or null.
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads)
     permute_quantize_kernel(uint2* __restrict__ codes, uint8_t* __restrict__ scales,
                             const __nv_bfloat16* __restrict__ hidden,
                             const int32_t* __restrict__ s2d, const float* __restrict__ global,
-                            int topk, int row_blocks) {
+                            int topk, int row_blocks, int32_t* __restrict__ zero, int zeros) {
   const int64_t t = blockIdx.x;
+  if (zero != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < zeros)
+    zero[threadIdx.x] = 0;
   const int b = blockIdx.y * kThreads + threadIdx.x;
   if (b >= row_blocks) return;
   const float g = global ? __ldg(global) : 1.0f;
@@ -185,7 +175,7 @@ lsek_status quantize_t(void* codes, void* scales, const void* x, const float* gl
 // into the rows that src_to_dest_map gives.
 lsek_status launch_permute_quantize(void* codes, void* scales, const void* hidden,
                                     const int32_t* s2d, const float* global, int T, int topk,
-                                    int H, cudaStream_t st) {
+                                    int H, int32_t* zero, int zeros, cudaStream_t st) {
   const int row_blocks = H / kFp4Block;
   if (T == 0 || row_blocks == 0 || topk == 0) return LSEK_OK;
   const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(ceil_div(row_blocks, kThreads)));
@@ -193,9 +183,11 @@ lsek_status launch_permute_quantize(void* codes, void* scales, const void* hidde
   uint8_t* s = static_cast<uint8_t*>(scales);
   const __nv_bfloat16* in = static_cast<const __nv_bfloat16*>(hidden);
   if (aligned(hidden, 32))
-    permute_quantize_kernel<true><<<grid, kThreads, 0, st>>>(c, s, in, s2d, global, topk, row_blocks);
+    permute_quantize_kernel<true><<<grid, kThreads, 0, st>>>(c, s, in, s2d, global, topk, row_blocks,
+                                                        zero, zeros);
   else
-    permute_quantize_kernel<false><<<grid, kThreads, 0, st>>>(c, s, in, s2d, global, topk, row_blocks);
+    permute_quantize_kernel<false><<<grid, kThreads, 0, st>>>(c, s, in, s2d, global, topk, row_blocks,
+                                                        zero, zeros);
   return check_launch("moe_permute_nvfp4");
 }
 
@@ -272,5 +264,6 @@ extern "C" lsek_status lsek_moe_permute_nvfp4(void* codes, void* scales, int32_t
                                        num_tokens, topk, num_experts, stream);
   if (s != LSEK_OK || empty) return s;
   return launch_permute_quantize(codes, scales, hidden_states, src_to_dest_map, global_scale,
-                                 num_tokens, topk, hidden_dim, static_cast<cudaStream_t>(stream));
+                                 num_tokens, topk, hidden_dim, nullptr, 0,
+                                 static_cast<cudaStream_t>(stream));
 }

@@ -19,8 +19,8 @@
 // most kTokRows.  Units are (expert, n-tile, chunk), chunk fastest, so chunks
 // that share a weight tile are taken at about the same time by neighbouring
 // CTAs and the weight tile comes from HBM once.  A persistent grid of one CTA
-// per SM takes units from an atomic counter in caller scratch, or with a
-// static stride where there is none.
+// per SM: CTA i starts with unit i and takes its further ones from an atomic
+// counter in caller scratch, or with a static stride where there is none.
 //
 // K runs in stages of 256 elements: one 128-byte swizzled row of codes, four
 // MMAs of K=64, and 16 scale bytes a row.  The MMA reads scales from TMEM,
@@ -43,12 +43,12 @@
 //   warp 1       MMA issuer: 4 x 2 MMAs a stage
 //   warps 2-9    epilogue, two groups of four (warp w reads TMEM lanes
 //                32*(w%4)..+31 = its 32 weight rows; the groups alternate
-//                chunks of 16 tokens).  A warp first drains its part of the
-//                tile into registers as bf16 pairs of the two boxes (g and u,
-//                or columns c and c + 128) and gives the accumulator back,
-//                then turns each 16 x 32 piece in shared memory so that a lane
-//                holds 16 consecutive outputs of one token: one 32-byte bf16
-//                store, or one NVFP4 block
+//                chunks of 16 tokens).  A chunk comes out of TMEM as bf16 pairs
+//                of the two boxes (g and u, or columns c and c + 128), the next
+//                one's load under its arithmetic.  bf16 outputs go straight to
+//                memory (64 bytes of a token a store); for NVFP4 outputs the
+//                warp turns its 16 x 32 piece in shared memory, so that a lane
+//                holds one block of 16 outputs of a token
 //   warps 10-13  scales: shared memory -> TMEM
 //   warp 14      TMA producer of the tokens' codes
 //   warp 15      TMA producer of scales, into a ring of their own: they are in
@@ -93,7 +93,6 @@ constexpr int kStagePitch = 80;                   // epilogue: bytes of a token'
 
 constexpr int kTok = 192;                         // most token rows of a unit
 constexpr int kHalves = 2;                        // 128-row scale tiles of the tokens
-constexpr int kChunks = kTok / 32;                // 16-token chunks of an epilogue group
 constexpr int kRecs = 8;                          // stages in flight at most
 constexpr int kSfStages = 3;
 constexpr int kSfTokOff = 2 * kSfBoxBytes;        // token scales, 16 bytes a row
@@ -197,7 +196,7 @@ struct Params {
   int out_tile_cols;       // output columns per tile
   int n_out;
   float swiglu_limit;
-  int32_t* counter;        // zeroed unit counter, or null (static stride)
+  int32_t* counter;        // zeroed counter of the units past the first of each CTA, or null
   int sf_by_tma;           // rows of a_sf are multiples of 16 bytes (K % 256 == 0)
 };
 
@@ -210,26 +209,42 @@ struct Maps {
 
 // ---- PTX ----------------------------------------------------------------------
 
-// mbar_wait with its first try inline: the call alone costs hundreds of cycles
-// in a chain that has a wait in every link.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int32_t* abort,
-                                         int32_t code) {
-  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort, code, true);
+// mbar_wait for chains that have a wait in every link: the first try is inline
+// (the call costs hundreds of cycles even on a completed barrier), and later
+// ones let the hardware suspend the warp for up to 20 us, so that waiting warps
+// leave the issue slots to the epilogue.
+__device__ __forceinline__ bool wait_bar_slow(uint64_t* bar, uint32_t parity,
+                                              volatile int32_t* abort, int32_t code,
+                                              bool honor_abort) {
+  const uint64_t t0 = global_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (honor_abort && *abort) return false;
+    if (global_ns() - t0 > kWaitLimitNs) {
+      *abort = 1;
+      report_device_error(code);
+      return false;
+    }
+  }
 }
-
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int32_t* abort,
+                                         int32_t code, bool honor_abort = true) {
+  return mbar_try_wait(bar, parity) || wait_bar_slow(bar, parity, abort, code, honor_abort);
+}
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
           smem_u32(dst)),
       "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
-}
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7])
-      : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -427,15 +442,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       RingPos<G> pos;
       uint32_t j_free = 0, held = 0;
+      int next = blockIdx.x;
       for (uint32_t qn = 0; ok; ++qn) {
         const int qslot = qn % kUnitQ;
         if (!wait_bar(&s.q_empty[qslot], ((qn / kUnitQ) & 1u) ^ 1u, abort, kDevErrGemmProducerWait)) {
           ok = false;
           break;
         }
-        int unit = p.counter ? atomicAdd(p.counter, 1)
-                             : static_cast<int>(blockIdx.x + qn * gridDim.x);
-        if (unit >= total) unit = -1;
+        const int unit = next < total ? next : -1;
         s.unit_q[qslot] = unit;
         mbar_arrive(&s.q_full[qslot]);
         if (unit < 0) break;
@@ -444,6 +458,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tok_bytes = ((u.rows + 15) & ~15) * kRowBytes;
         const int brow = u.e * p.b_rows + u.n * p.b_tile_rows;
         for (int kb = 0; kb < num_kb; ++kb, ++pos.j) {
+          // The next unit is asked for a few stages early, so that the answer is
+          // there when this one's loads have been issued.
+          if (kb == max(0, num_kb - 3))
+            next = gridDim.x + (p.counter ? atomicAdd(p.counter, 1) : unit);
           const uint32_t span = pos.layout(boxes, tok_bytes);
           if (!reserve(s.span[0], pos.j, span, j_free, held)) {
             ok = false;
@@ -458,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) {  // let every issued load land before the CTA can exit
         for (uint32_t d = j_free; d < pos.j; ++d)
-          mbar_wait(&s.full_bar[d % kRecs], (d / kRecs) & 1u, abort, kDevErrGemmProducerWait, false);
+          wait_bar(&s.full_bar[d % kRecs], (d / kRecs) & 1u, abort, kDevErrGemmProducerWait, false);
       }
     }
   } else if (warp == kTokWarp) {
@@ -498,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) {
         for (uint32_t d = j_free; d < pos.j; ++d)
-          mbar_wait(&s.full_bar[d % kRecs], (d / kRecs) & 1u, abort, kDevErrGemmProducerWait, false);
+          wait_bar(&s.full_bar[d % kRecs], (d / kRecs) & 1u, abort, kDevErrGemmProducerWait, false);
       }
     }
   } else if (warp == kSfLoadWarp) {
@@ -547,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) {
         for (uint32_t d = j > kSfStages ? j - kSfStages : 0; d < j; ++d)
-          mbar_wait(&s.sf_full_bar[d % kSfStages], (d / kSfStages) & 1u, abort, kDevErrGemmScaleWait, false);
+          wait_bar(&s.sf_full_bar[d % kSfStages], (d / kSfStages) & 1u, abort, kDevErrGemmScaleWait, false);
       }
     }
   } else if (warp == 1) {
@@ -610,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // Outstanding MMAs read shared memory and write TMEM: finish them first.
       umma_commit(&s.mma_done_bar);
-      mbar_wait(&s.mma_done_bar, 0, abort, kDevErrGemmMmaWait, false);
+      wait_bar(&s.mma_done_bar, 0, abort, kDevErrGemmMmaWait, false);
     }
   } else if (warp >= kFirstSfWarp && warp < kTokWarp) {
     // ===================== scales (warps 10..13) =====================
@@ -732,69 +750,64 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tok = lane >> 1;                  // after the turn: token and
       const int feat = q * 32 + (lane & 1) * 16;  // first of 16 output columns of the box
       const uint4* mine = reinterpret_cast<const uint4*>(turn + tok * kStagePitch + (lane & 1) * 32);
-      // Drain: both boxes as a bf16 pair for each token of this warp's chunks.
-      uint32_t pair[kChunks][16];
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int t0 = (2 * c + grp) * 16;
-        if (t0 < nn) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 8) {
-            uint32_t v0[8], v1[8];
-            tmem_ld8(d0 + t0 + i, v0);
-            tmem_ld8(d1 + t0 + i, v1);  // not written by a unit with one box; not used then
-            tmem_ld_wait();
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              pair[c][i + x] = pack_bf16x2(__fmul_rn(alpha, __uint_as_float(v0[x])),
-                                           __fmul_rn(alpha, __uint_as_float(v1[x])));
-          }
+      auto give_back = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.acc_empty_bar[acc0]);
+          if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
         }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&s.acc_empty_bar[acc0]);
-        if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
-      }
+      };
+      // Chunks of 16 tokens: g and u (or both boxes' columns) as bf16 pairs; the
+      // next chunk's TMEM loads run under this one's arithmetic, and the
+      // accumulator goes back before the last chunk's.
+      uint32_t v0[16], v1[16], pair[16];
+      auto load_chunk = [&](int t0) {
+        tmem_ld16(d0 + t0, v0);
+        tmem_ld16(d1 + t0, v1);  // not written by a unit with one box; not used then
+      };
+      if (grp * 16 < nn) load_chunk(grp * 16);
+#pragma unroll 1
+      for (int t0 = grp * 16; t0 < nn; t0 += 32) {
+        tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int t0 = (2 * c + grp) * 16;
-        if (t0 >= nn) break;
-        const int64_t row = u.row0 + t0 + tok;
-        const bool live = t0 + tok < u.rows;
+        for (int i = 0; i < 16; ++i)
+          pair[i] = pack_bf16x2(__fmul_rn(alpha, __uint_as_float(v0[i])),
+                                __fmul_rn(alpha, __uint_as_float(v1[i])));
+        if (t0 + 32 < nn) load_chunk(t0 + 32);
+        else give_back();
+        if (SWIGLU) {
 #pragma unroll
-        for (int b = 0; b < (SWIGLU ? 1 : 2); ++b) {
-          if (b == 1 && boxes == 1) break;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            uint16_t h;
-            if (SWIGLU)
-              h = __bfloat16_as_ushort(__float2bfloat16_rn(
-                  swiglu_f32(__uint_as_float(pair[c][i] << 16),
-                             __uint_as_float(pair[c][i] & 0xFFFF0000u), p.swiglu_limit)));
-            else
-              h = static_cast<uint16_t>(b == 0 ? pair[c][i] : pair[c][i] >> 16);
-            *reinterpret_cast<uint16_t*>(turn + i * kStagePitch + lane * 2) = h;
-          }
+          for (int i = 0; i < 16; ++i)
+            *reinterpret_cast<__nv_bfloat16*>(turn + i * kStagePitch + lane * 2) =
+                __float2bfloat16_rn(swiglu_f32(__uint_as_float(pair[i] << 16),
+                                               __uint_as_float(pair[i] & 0xFFFF0000u),
+                                               p.swiglu_limit));
           __syncwarp();
           const uint4 lo = mine[0], hi = mine[1];
           __syncwarp();
-          const int f = b * kBoxRows + feat;
-          if (live && f < cols) {
-            if (SWIGLU) {
-              const Fp4Block blk = fp4_quantize16<__nv_bfloat16>(lo, hi, go, six_go);
-              const int64_t at = (row * p.n_out + col0 + f) / kFp4Block;
-              reinterpret_cast<uint2*>(p.out_codes)[at] = blk.codes;
-              p.out_sf[at] = static_cast<uint8_t>(blk.scale);
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(p.D + row * p.n_out + col0 + f);
-              dst[0] = lo;
-              dst[1] = hi;
+          if (t0 + tok < u.rows && feat < cols) {
+            const Fp4Block blk = fp4_quantize16<__nv_bfloat16>(lo, hi, go, six_go);
+            const int64_t at = (static_cast<int64_t>(u.row0 + t0 + tok) * p.n_out + col0 + feat) / kFp4Block;
+            reinterpret_cast<uint2*>(p.out_codes)[at] = blk.codes;
+            p.out_sf[at] = static_cast<uint8_t>(blk.scale);
+          }
+        } else {
+          // A token's 32 columns of this warp are one 64-byte store.
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.D) +
+                          static_cast<int64_t>(u.row0 + t0) * p.n_out + col0 + q * 32 + lane;
+          const bool in0 = q * 32 + lane < cols, in1 = kBoxRows + q * 32 + lane < cols;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (t0 + i < u.rows) {
+              if (in0) dst[0] = static_cast<uint16_t>(pair[i]);
+              if (in1) dst[kBoxRows] = static_cast<uint16_t>(pair[i] >> 16);
             }
+            dst += p.n_out;
           }
         }
       }
+      if (grp * 16 >= nn) give_back();
       ac += two ? 2u : 1u;
     }
   }
@@ -833,7 +846,8 @@ lsek_status make_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_
 }
 
 template <bool SWIGLU, class G>
-lsek_status launch_geom(Params p, const void* A, const void* B, int K, cudaStream_t st) {
+lsek_status launch_geom(Params p, const void* A, const void* B, int K, bool zero_counter,
+                        cudaStream_t st) {
   static PerDeviceOnce attrs;
   const cudaError_t ae = once_per_device(attrs, [] {
     return cudaFuncSetAttribute(fp4_gemm_kernel<SWIGLU, G>,
@@ -851,11 +865,15 @@ lsek_status launch_geom(Params p, const void* A, const void* B, int K, cudaStrea
       s = make_map(&m.s[i], p.a_sf, row_bytes / 8, static_cast<uint64_t>(p.rows), 16u << i, 16u);
   }
   if (s != LSEK_OK) return s;
-  if (p.counter != nullptr) LSEK_CUDA_TRY(cudaMemsetAsync(p.counter, 0, sizeof(int32_t), st));
   // At most rows / kTok full chunks and one partial chunk per non-empty expert.
   const int64_t experts = p.num_experts < p.rows ? p.num_experts : p.rows;
   const int64_t max_units = (p.rows / kTok + experts) * static_cast<int64_t>(p.n_tiles);
   const int grid = static_cast<int>(max_units < num_sms() ? max_units : num_sms());
+  // No expert of more than kTok rows: the units are alike (each streams one
+  // weight tile), and a static stride does without the memset (2 us).
+  if (p.rows <= kTok) p.counter = nullptr;
+  if (p.counter != nullptr && zero_counter)
+    LSEK_CUDA_TRY(cudaMemsetAsync(p.counter, 0, sizeof(int32_t), st));
   fp4_gemm_kernel<SWIGLU, G><<<grid, kThreads, smem_bytes<G>(), st>>>(m, p);
   return check_launch(SWIGLU ? "grouped_gemm_swiglu_nvfp4" : "grouped_gemm_nvfp4");
 }
@@ -870,12 +888,13 @@ lsek_status fp4_take_device_error(int32_t* code) {
 }
 
 // Both products; D for the plain one, h_codes / h_scales for gate/up + SwiGLU
-// (n_out = I there).  Every argument has been checked.
+// (n_out = I there).  Every argument has been checked.  counter: an int32 of
+// device scratch, or null; zero_counter: it has to be zeroed here.
 lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales, const void* A,
                              const void* a_scales, const void* B, const void* b_tiles,
                              const int32_t* offsets, const float* a_global, const float* b_global,
                              const float* out_global, int E, int rows, int n_out, int K,
-                             float limit, int32_t* counter, cudaStream_t st) {
+                             float limit, int32_t* counter, bool zero_counter, cudaStream_t st) {
   using namespace fp4;
   if (rows == 0 || n_out == 0) return LSEK_OK;
   Params p{};
@@ -915,10 +934,10 @@ lsek_status grouped_gemm_fp4(bool swiglu, void* D, void* h_codes, void* h_scales
   }
   p.n_tiles = static_cast<int>(ceil_div(n_out, p.out_tile_cols));
   if (E <= GeomFull::kMaxE)
-    return swiglu ? launch_geom<true, GeomFull>(p, A, B, K, st)
-                  : launch_geom<false, GeomFull>(p, A, B, K, st);
-  return swiglu ? launch_geom<true, GeomWide>(p, A, B, K, st)
-                : launch_geom<false, GeomWide>(p, A, B, K, st);
+    return swiglu ? launch_geom<true, GeomFull>(p, A, B, K, zero_counter, st)
+                  : launch_geom<false, GeomFull>(p, A, B, K, zero_counter, st);
+  return swiglu ? launch_geom<true, GeomWide>(p, A, B, K, zero_counter, st)
+                : launch_geom<false, GeomWide>(p, A, B, K, zero_counter, st);
 }
 
 namespace {
@@ -966,7 +985,7 @@ extern "C" lsek_status lsek_grouped_gemm_nvfp4(void* D, const void* A, const voi
   if (s != LSEK_OK) return s;
   return grouped_gemm_fp4(false, D, nullptr, nullptr, A, a_scales, B, b_scale_tiles, expert_offsets,
                           a_global_scale, b_global_scale, nullptr, num_experts, rows, N, K, 0.0f,
-                          counter_in(workspace, workspace_bytes), static_cast<cudaStream_t>(stream));
+                          counter_in(workspace, workspace_bytes), true, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" lsek_status lsek_grouped_gemm_swiglu_nvfp4(
@@ -984,6 +1003,6 @@ extern "C" lsek_status lsek_grouped_gemm_swiglu_nvfp4(
   LSEK_REQUIRE(swiglu_limit >= 0.0f, "grouped_gemm_swiglu_nvfp4: swiglu_limit must be >= 0");
   return grouped_gemm_fp4(true, nullptr, h_codes, h_scales, A, a_scales, W_gu, gu_scale_tiles,
                           expert_offsets, a_global_scale, gu_global_scale, h_global_scale,
-                          num_experts, rows, I, K, swiglu_limit, counter_in(workspace, workspace_bytes),
+                          num_experts, rows, I, K, swiglu_limit, counter_in(workspace, workspace_bytes), true,
                           static_cast<cudaStream_t>(stream));
 }
