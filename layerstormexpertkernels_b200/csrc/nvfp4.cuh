@@ -65,6 +65,36 @@ __device__ __forceinline__ float2 e2m1x2_to_f32(uint32_t byte) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h2));
 }
 
+// Two fp32 products in one instruction, each rounded once.
+__device__ __forceinline__ float2 mul_f32x2(float a0, float a1, float b0, float b1) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 c, a, b;\n\t"
+      "mov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+  return r;
+}
+
+// Pairs of 16-bit values: |x|, the larger of two (NaN if either is), and fp32.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7FFF7FFFu), "r"(b & 0x7FFF7FFFu));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b, __half) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7FFF7FFFu), "r"(b & 0x7FFF7FFFu));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 struct Fp4Block {
   uint2 codes;     // 16 codes, element i in bits 4i of the 64
   uint32_t scale;  // E4M3 bits
@@ -76,12 +106,10 @@ template <typename T>
 __device__ __forceinline__ Fp4Block fp4_quantize16(const uint4& lo, const uint4& hi, float g,
                                                    float six_g) {
   const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-  // The order of magnitudes is the order of the bits without the sign,
-  // infinities and NaNs above every finite value.
-  uint32_t m = w[0] & 0x7FFF7FFFu;
+  uint32_t m = max_abs2(w[0], w[1], T());
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-  const uint32_t amax_bits = max(m & 0xFFFFu, m >> 16);
+  for (int i = 2; i < 8; ++i) m = max_abs2(m, w[i], T());
+  const uint32_t amax_bits = max_abs2(m, m >> 16, T()) & 0xFFFFu;
   const uint16_t ab = static_cast<uint16_t>(amax_bits);
   const float amax = Elem<T>::to_f(*reinterpret_cast<const T*>(&ab));
   Fp4Block q;
@@ -94,9 +122,10 @@ __device__ __forceinline__ Fp4Block fp4_quantize16(const uint4& lo, const uint4&
     float y[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const T* e = reinterpret_cast<const T*>(&w[4 * h + i]);
-      y[2 * i] = __fmul_rn(Elem<T>::to_f(e[0]), inv);
-      y[2 * i + 1] = __fmul_rn(Elem<T>::to_f(e[1]), inv);
+      const float2 x = unpack2(w[4 * h + i], T());
+      const float2 p = mul_f32x2(x.x, x.y, inv, inv);
+      y[2 * i] = p.x;
+      y[2 * i + 1] = p.y;
     }
     half[h] = e2m1x8_from_f32(y);
   }

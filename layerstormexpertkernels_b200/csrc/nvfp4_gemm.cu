@@ -289,6 +289,39 @@ __device__ __forceinline__ uint32_t fp4_idesc(int nn) {
          (static_cast<uint32_t>(kBoxRows >> 7) << 27);
 }
 
+// h = bf16(silu(g) u) of 16 tokens (bf16 pairs) of this lane's column, into the
+// turning buffer.  The arithmetic of swiglu_f32, silu(g) = g / (1 + 2^(-g
+// log2 e)), two tokens an instruction where there is one and with the
+// flush-to-zero forms of the exponential and the reciprocal: half its
+// instructions, which bound this epilogue.  Results that are bf16 subnormals
+// may come out as zeros of the same sign, which quantise to the same codes
+// (their quotients are below 2^-17); all others have swiglu_f32's bits, tried for
+// every bf16 g.
+template <bool CLAMP>
+__device__ __forceinline__ void swiglu_turn(const uint32_t (&g2)[8], const uint32_t (&u2)[8],
+                                            float limit, uint8_t* turn, int lane) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float2 g = unpack2(g2[i], __nv_bfloat16()), u = unpack2(u2[i], __nv_bfloat16());
+    if (CLAMP) {
+      g = make_float2(fminf(g.x, limit), fminf(g.y, limit));
+      u = make_float2(fminf(fmaxf(u.x, -limit), limit), fminf(fmaxf(u.y, -limit), limit));
+    }
+    const float2 t = mul_f32x2(g.x, g.y, -1.4426950408889634f, -1.4426950408889634f);
+    float e0, e1, r0, r1;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t.y));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(__fadd_rn(1.0f, e0)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(__fadd_rn(1.0f, e1)));
+    const float2 s = mul_f32x2(g.x, g.y, r0, r1);
+    const float2 h = mul_f32x2(s.x, s.y, u.x, u.y);
+    const uint32_t pair = pack_bf16x2(h.x, h.y);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(turn + 2 * i * kStagePitch) + lane;
+    dst[0] = static_cast<uint16_t>(pair);
+    dst[kStagePitch / 2] = static_cast<uint16_t>(pair >> 16);
+  }
+}
+
 // ---- work units -----------------------------------------------------------------
 
 template <class S>
@@ -758,50 +791,52 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (two) mbar_arrive(&s.acc_empty_bar[acc1]);
         }
       };
-      // Chunks of 16 tokens: g and u (or both boxes' columns) as bf16 pairs; the
-      // next chunk's TMEM loads run under this one's arithmetic, and the
-      // accumulator goes back before the last chunk's.
-      uint32_t v0[16], v1[16], pair[16];
+      // Chunks of 16 tokens.  A chunk's accumulators are scaled and rounded to
+      // bf16 pairs of tokens; then the next chunk's TMEM loads start (or the
+      // accumulator goes back) and run under this one's arithmetic.
+      uint32_t v0[16], v1[16], p0[8], p1[8];
       auto load_chunk = [&](int t0) {
         tmem_ld16(d0 + t0, v0);
         tmem_ld16(d1 + t0, v1);  // not written by a unit with one box; not used then
       };
       if (grp * 16 < nn) load_chunk(grp * 16);
+      const int64_t row0 = u.row0 + grp * 16;
+      // SWIGLU: this lane's block of token row0 + tok; else column q * 32 + lane of row0
+      int64_t at = SWIGLU ? ((row0 + tok) * p.n_out + col0 + feat) / kFp4Block
+                          : row0 * p.n_out + col0 + q * 32 + lane;
+      const int64_t at_step = SWIGLU ? 2 * p.n_out : 32ll * p.n_out;  // 32 rows on
+      const bool in0 = (SWIGLU ? feat : q * 32 + lane) < cols, in1 = kBoxRows + q * 32 + lane < cols;
 #pragma unroll 1
-      for (int t0 = grp * 16; t0 < nn; t0 += 32) {
+      for (int t0 = grp * 16; t0 < nn; t0 += 32, at += at_step) {
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          pair[i] = pack_bf16x2(__fmul_rn(alpha, __uint_as_float(v0[i])),
-                                __fmul_rn(alpha, __uint_as_float(v1[i])));
+        for (int i = 0; i < 8; ++i) {
+          const float2 a = mul_f32x2(__uint_as_float(v0[2 * i]), __uint_as_float(v0[2 * i + 1]), alpha, alpha);
+          const float2 b = mul_f32x2(__uint_as_float(v1[2 * i]), __uint_as_float(v1[2 * i + 1]), alpha, alpha);
+          p0[i] = pack_bf16x2(a.x, a.y);
+          p1[i] = pack_bf16x2(b.x, b.y);
+        }
         if (t0 + 32 < nn) load_chunk(t0 + 32);
         else give_back();
         if (SWIGLU) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            *reinterpret_cast<__nv_bfloat16*>(turn + i * kStagePitch + lane * 2) =
-                __float2bfloat16_rn(swiglu_f32(__uint_as_float(pair[i] << 16),
-                                               __uint_as_float(pair[i] & 0xFFFF0000u),
-                                               p.swiglu_limit));
+          if (p.swiglu_limit > 0.0f) swiglu_turn<true>(p0, p1, p.swiglu_limit, turn, lane);
+          else swiglu_turn<false>(p0, p1, 0.0f, turn, lane);
           __syncwarp();
           const uint4 lo = mine[0], hi = mine[1];
           __syncwarp();
-          if (t0 + tok < u.rows && feat < cols) {
+          if (t0 + tok < u.rows && in0) {
             const Fp4Block blk = fp4_quantize16<__nv_bfloat16>(lo, hi, go, six_go);
-            const int64_t at = (static_cast<int64_t>(u.row0 + t0 + tok) * p.n_out + col0 + feat) / kFp4Block;
             reinterpret_cast<uint2*>(p.out_codes)[at] = blk.codes;
             p.out_sf[at] = static_cast<uint8_t>(blk.scale);
           }
         } else {
           // A token's 32 columns of this warp are one 64-byte store.
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.D) +
-                          static_cast<int64_t>(u.row0 + t0) * p.n_out + col0 + q * 32 + lane;
-          const bool in0 = q * 32 + lane < cols, in1 = kBoxRows + q * 32 + lane < cols;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.D) + at;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             if (t0 + i < u.rows) {
-              if (in0) dst[0] = static_cast<uint16_t>(pair[i]);
-              if (in1) dst[kBoxRows] = static_cast<uint16_t>(pair[i] >> 16);
+              if (in0) dst[0] = static_cast<uint16_t>(p0[i / 2] >> (16 * (i & 1)));
+              if (in1) dst[kBoxRows] = static_cast<uint16_t>(p1[i / 2] >> (16 * (i & 1)));
             }
             dst += p.n_out;
           }
