@@ -801,9 +801,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (grp * 16 < nn) load_chunk(grp * 16);
       const int64_t row0 = u.row0 + grp * 16;
-      // SWIGLU: this lane's block of token row0 + tok; else column q * 32 + lane of row0
+      // SWIGLU: this lane's block of token row0 + tok; else its two columns of the
+      // first or second row of a pair
       int64_t at = SWIGLU ? ((row0 + tok) * p.n_out + col0 + feat) / kFp4Block
-                          : row0 * p.n_out + col0 + q * 32 + lane;
+                          : (row0 + (lane & 1)) * p.n_out + col0 + q * 32 + (lane & ~1);
+      const uint32_t trade = (lane & 1) == 0 ? 0x5410u : 0x3276u;
       const int64_t at_step = SWIGLU ? 2 * p.n_out : 32ll * p.n_out;  // 32 rows on
       const bool in0 = (SWIGLU ? feat : q * 32 + lane) < cols, in1 = kBoxRows + q * 32 + lane < cols;
 #pragma unroll 1
@@ -830,15 +832,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.out_sf[at] = static_cast<uint8_t>(blk.scale);
           }
         } else {
-          // A token's 32 columns of this warp are one 64-byte store.
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.D) + at;
+          // Neighbouring lanes trade, so that an even lane has two columns of the
+          // even token of a pair and an odd lane those of the odd one.
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (t0 + i < u.rows) {
-              if (in0) dst[0] = static_cast<uint16_t>(p0[i / 2] >> (16 * (i & 1)));
-              if (in1) dst[kBoxRows] = static_cast<uint16_t>(p1[i / 2] >> (16 * (i & 1)));
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t o0 = __shfl_xor_sync(0xffffffffu, p0[i], 1);
+            const uint32_t o1 = __shfl_xor_sync(0xffffffffu, p1[i], 1);
+            if (t0 + 2 * i + (lane & 1) < u.rows) {
+              __nv_bfloat16* dst = p.D + at + 2 * i * p.n_out;
+              if (in0) *reinterpret_cast<uint32_t*>(dst) = __byte_perm(p0[i], o0, trade);
+              if (in1) *reinterpret_cast<uint32_t*>(dst + kBoxRows) = __byte_perm(p1[i], o1, trade);
             }
-            dst += p.n_out;
           }
         }
       }
