@@ -8,6 +8,7 @@
 // INVALID_ARG raises ValueError, every other failure RuntimeError, as the
 // reference's launchers do via pybind11's exception translation.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime_api.h>
 #include <pybind11/stl.h>
@@ -408,6 +409,11 @@ void moe_layer_forward_out(torch::Tensor out, torch::Tensor hidden, torch::Tenso
 
 // ---- NVFP4 experts -------------------------------------------------------------
 
+// torch::empty without the dispatcher, which takes half of a small call's host time.
+torch::Tensor new_tensor(at::IntArrayRef shape, at::ScalarType dtype, const torch::Tensor& like) {
+  return torch::Tensor(at::detail::empty_cuda(shape, dtype, like.device(), c10::nullopt));
+}
+
 // One float32 on the device for each of n groups; absent means 1.
 const float* global_ptr(const char* op, const char* what, const c10::optional<torch::Tensor>& g,
                         int64_t n, const torch::Tensor& like) {
@@ -463,9 +469,9 @@ std::vector<torch::Tensor> nvfp4_quantize(torch::Tensor x, c10::optional<torch::
   const float* g = global_ptr(op, "global_scale", global_scale, r.groups, x);
   auto shape = x.sizes().vec();
   shape.back() = r.k / 2;
-  auto codes = torch::empty(shape, x.options().dtype(at::kByte));
+  auto codes = new_tensor(shape, at::kByte, x);
   shape.back() = r.k / 16;
-  auto scales = torch::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  auto scales = new_tensor(shape, at::kFloat8_e4m3fn, x);
   check_status(lsek_nvfp4_quantize(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), g, r.groups,
                                    r.rows, to_i32(r.k, "K"), dtype_code(x), stream_of(x)));
   return {codes, scales};
@@ -484,7 +490,7 @@ torch::Tensor nvfp4_dequantize(torch::Tensor codes, torch::Tensor scales,
   const float* g = global_ptr(op, "global_scale", global_scale, r.groups, codes);
   auto shape = codes.sizes().vec();
   shape.back() = 2 * r.k;
-  auto out = torch::empty(shape, codes.options().dtype(dtype));
+  auto out = new_tensor(shape, dtype, codes);
   check_status(lsek_nvfp4_dequantize(out.data_ptr(), codes.data_ptr(), scales.data_ptr(), g, r.groups,
                                      r.rows, to_i32(2 * r.k, "K"), dtype_code(out),
                                      stream_of(codes)));
@@ -512,11 +518,11 @@ std::vector<torch::Tensor> moe_permute_nvfp4(torch::Tensor hidden_states, torch:
   const c10::cuda::OptionalCUDAGuard guard(hidden_states.device());
   const float* g = global_ptr(op, "global_scale", global_scale, 1, hidden_states);
   const int64_t n = T * k;
-  auto codes = torch::empty({n, H / 2}, hidden_states.options().dtype(at::kByte));
-  auto scales = torch::empty({n, H / 16}, hidden_states.options().dtype(at::kFloat8_e4m3fn));
-  auto offsets = torch::empty({num_experts + 1}, topk_indices.options());
-  auto s2d = torch::empty({n}, topk_indices.options());
-  auto perm = torch::empty({n}, topk_indices.options());
+  auto codes = new_tensor({n, H / 2}, at::kByte, hidden_states);
+  auto scales = new_tensor({n, H / 16}, at::kFloat8_e4m3fn, hidden_states);
+  auto offsets = new_tensor({num_experts + 1}, at::kInt, topk_indices);
+  auto s2d = new_tensor({n}, at::kInt, topk_indices);
+  auto perm = new_tensor({n}, at::kInt, topk_indices);
   check_status(lsek_moe_permute_nvfp4(
       codes.data_ptr(), scales.data_ptr(), offsets.data_ptr<int32_t>(), s2d.data_ptr<int32_t>(),
       perm.data_ptr<int32_t>(), hidden_states.data_ptr(), topk_indices.data_ptr<int32_t>(), g,
@@ -562,8 +568,8 @@ torch::Tensor grouped_gemm_nvfp4(torch::Tensor A, torch::Tensor A_scales, torch:
   const c10::cuda::OptionalCUDAGuard guard(A.device());
   const float* ga = global_ptr(op, "a_global_scale", a_global_scale, 1, A);
   const float* gb = global_ptr(op, "b_global_scale", b_global_scale, B.size(0), A);
-  auto D = torch::empty({A.size(0), B.size(1)}, A.options().dtype(at::kBFloat16));
-  auto ws = torch::empty({LSEK_GEMM_WORKSPACE_BYTES}, A.options());
+  auto D = new_tensor({A.size(0), B.size(1)}, at::kBFloat16, A);
+  auto ws = new_tensor({LSEK_GEMM_WORKSPACE_BYTES}, at::kByte, A);
   check_status(lsek_grouped_gemm_nvfp4(
       D.data_ptr(), A.data_ptr(), A_scales.data_ptr(), B.data_ptr(), B_scales.data_ptr(),
       expert_offsets.data_ptr<int32_t>(), ga, gb, to_i32(B.size(0), "E"), to_i32(A.size(0), "rows"),
@@ -586,9 +592,9 @@ std::vector<torch::Tensor> grouped_gemm_swiglu_nvfp4(
   const float* go = global_ptr(op, "out_global_scale", out_global_scale, 1, A);
   const int64_t I = W_gu.size(1) / 2;
   TORCH_CHECK(I % 32 == 0, op, ": I must be a multiple of 32, got ", I);
-  auto codes = torch::empty({A.size(0), I / 2}, A.options());
-  auto scales = torch::empty({A.size(0), I / 16}, A_scales.options());
-  auto ws = torch::empty({LSEK_GEMM_WORKSPACE_BYTES}, A.options());
+  auto codes = new_tensor({A.size(0), I / 2}, at::kByte, A);
+  auto scales = new_tensor({A.size(0), I / 16}, at::kFloat8_e4m3fn, A);
+  auto ws = new_tensor({LSEK_GEMM_WORKSPACE_BYTES}, at::kByte, A);
   check_status(lsek_grouped_gemm_swiglu_nvfp4(
       codes.data_ptr(), scales.data_ptr(), A.data_ptr(), A_scales.data_ptr(), W_gu.data_ptr(),
       W_gu_scales.data_ptr(), expert_offsets.data_ptr<int32_t>(), ga, gw, go,
