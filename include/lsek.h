@@ -266,7 +266,8 @@ LSEK_API lsek_status lsek_grouped_gemm_swiglu_bf16(void* Hout, const void* A,
 /* An NVFP4 tensor of rows of K elements is
  *   codes  [rows, K/2] uint8: two E2M1 codes a byte, the even element in the
  *          low nibble (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 is the sign)
- *   scales [rows, K/16] E4M3: one for 16 consecutive elements of a row
+ *   scales [rows, K/16] E4M3, not negative: one for 16 consecutive elements
+ *          of a row
  *   global_scale: one float32 (per expert for weights), NULL for 1
  * and stands for code * scale * global_scale.  codes and scales are those of
  * ref_nvfp4_dequant (tests/test_reference.py:19-53); the reference's kernels
@@ -309,8 +310,8 @@ LSEK_API lsek_status lsek_moe_permute_nvfp4(void* codes, void* scales, int32_t* 
 /* lsek_grouped_gemm_bf16 on NVFP4 operands: A [rows, K] with row scales, B
  * [E, N, K] with tiled scales, D [rows, N] bf16 = the fp32 sum of the
  * products times a_global_scale * b_global_scale[e], rounded once.
- * K % 64 == 0, N % 32 == 0, tensors 16-byte aligned; expert_offsets and
- * workspace as there. */
+ * K % 64 == 0, N % 32 == 0, tensors 16-byte aligned (a_scales 4-byte);
+ * expert_offsets and workspace as there. */
 LSEK_API lsek_status lsek_grouped_gemm_nvfp4(void* D, const void* A, const void* a_scales,
                                     const void* B, const void* b_scale_tiles,
                                     const int32_t* expert_offsets, const float* a_global_scale,
@@ -321,7 +322,8 @@ LSEK_API lsek_status lsek_grouped_gemm_nvfp4(void* D, const void* A, const void*
 /* Gate/up product, SwiGLU and quantisation in one kernel: equal bit for bit to
  * lsek_grouped_gemm_nvfp4, lsek_fused_swiglu and lsek_nvfp4_quantize (with
  * h_global_scale) in a row.  W_gu [E, 2I, K]; h_codes [rows, I/2], h_scales
- * [rows, I/16].  K % 64 == 0, I % 32 == 0, tensors 16-byte aligned. */
+ * [rows, I/16].  K % 64 == 0, I % 32 == 0, tensors 16-byte aligned (a_scales
+ * 4-byte). */
 LSEK_API lsek_status lsek_grouped_gemm_swiglu_nvfp4(void* h_codes, void* h_scales, const void* A,
                                            const void* a_scales, const void* W_gu,
                                            const void* gu_scale_tiles,

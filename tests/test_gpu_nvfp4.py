@@ -286,6 +286,19 @@ def test_rows_of_an_expert_do_not_depend_on_their_neighbours():
     sync_and_check_device_error()
 
 
+def test_scales_that_start_at_a_4_byte_boundary():
+    """A row of scales is a multiple of 4 bytes, and so is a slice's start."""
+    P = pk()
+    a, asf, av, w, tiles, wv, off, d_off = make_product([5, 200], 160, 512, seed=40)
+    flat = torch.zeros(4 + asf.numel(), dtype=torch.uint8, device="cuda")
+    flat[4:] = asf.view(torch.uint8).flatten()
+    odd = flat[4:].view(torch.float8_e4m3fn).view(asf.shape)
+    assert odd.data_ptr() % 16 == 4
+    out = P.grouped_gemm_nvfp4(a, odd, w, tiles, d_off)
+    assert torch.equal(out, P.grouped_gemm_nvfp4(a, asf, w, tiles, d_off))
+    sync_and_check_device_error()
+
+
 def test_rows_behind_the_last_expert_stay():
     """Rows outside every expert are not written (C ABI, canary output), with
     and without the workspace."""
@@ -372,6 +385,163 @@ def test_swiglu_equals_product_swiglu_quantize(counts, inter, k, limit):
     err = (back - exact).abs().view(exact.shape[0], -1, 16).amax(-1)
     smallest = 0.02 * 2.0 ** -10 * 6  # below this amax a scale rounds to 0
     assert (err <= amax * (1 / 6 + 2.0 ** -4 + 2.0 ** -7 + 1e-3) + smallest).all()
+
+
+def test_swiglu_for_every_gate_value():
+    """Every bf16 gate magnitude and sign from 2^-126 up (128 significands as
+    columns, 18 exponents and both signs as tokens, 15 experts for the rest of
+    the exponents), with up values of the same exponent: the fused kernel's
+    arithmetic gives the codes of fused_swiglu's."""
+    P = pk()
+    inter, k = 128, 256
+    m = torch.arange(128, 256)
+    w = torch.zeros(2 * inter, k // 16)  # element 0 of block i: bit i of the significand
+    for i in range(8):
+        w[:inter, i] = ((m >> i) & 1) * 2.0 ** i
+    w[inter:, 8] = 128.0  # up row: 2^7, as the significand's top bit
+    codes = torch.zeros(2 * inter, k // 2, dtype=torch.uint8)
+    codes[:, ::8] = 2  # 1.0 at the first element of each block
+    tokens = torch.zeros(36, k // 2, dtype=torch.uint8)
+    tokens[:18, ::8], tokens[18:, ::8] = 2, 10
+    ascale = torch.exp2(torch.arange(-9, 9).float()).repeat(2)[:, None].repeat(1, k // 16)
+    E = 15
+    off = torch.arange(E + 1, dtype=torch.int32, device="cuda") * 36
+    gw = torch.exp2(torch.arange(E).float() * 18 - 124).cuda()
+    a = tokens.repeat(E, 1).cuda()
+    asf = ascale.repeat(E, 1).to(torch.float8_e4m3fn).cuda()
+    wc = codes[None].repeat(E, 1, 1).cuda()
+    wsf = w[None].repeat(E, 1, 1).to(torch.float8_e4m3fn).cuda()
+    two, one = P.nvfp4_tile_scales(wsf, 2), P.nvfp4_tile_scales(wsf, 1)
+    gu = P.grouped_gemm_nvfp4(a, asf, wc, one, off, None, gw)
+    g = gu[:, :inter].float()
+    finite = g[g.isfinite()]
+    assert finite.abs().unique().numel() > 128 * 250  # the sweep is one
+    for limit in (0.0, 10.0):
+        h = P.fused_swiglu(gu, swiglu_limit=limit)
+        for e in (-95, -60, -30, 0, 30, 60, 95):
+            go = glob(2.0 ** e)
+            got, got_s = P.grouped_gemm_swiglu_nvfp4(a, asf, wc, two, off, None, gw, go, swiglu_limit=limit)
+            want, want_s = P.nvfp4_quantize(h, go)
+            assert torch.equal(got_s.view(torch.uint8), want_s.view(torch.uint8))
+            assert torch.equal(got, want)
+    sync_and_check_device_error()
+
+
+def test_more_than_256_experts():
+    P = pk()
+    gen = torch.Generator().manual_seed(12)
+    counts = [int(c) for c in torch.randint(0, 4, (300,), generator=gen)]
+    counts[7] = 210
+    a, asf, av, w, tiles, wv, off, d_off = make_product(counts, 96, 128, seed=13)
+    out = P.grouped_gemm_nvfp4(a, asf, w, tiles, d_off)
+    sync_and_check_device_error()
+    assert_product(out, av, wv, off, [1.0] * 300)
+
+
+def test_no_expert_takes_a_row():
+    """Rows but empty experts (every slot pruned): nothing is written."""
+    P = pk()
+    a, asf, av, w, tiles, wv, off, d_off = make_product([0, 0, 0], 64, 128, seed=2, pad_rows=40)
+    lib = ctypes.CDLL(P.LIBRARY_PATH)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    d = torch.full((40, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+    st = lib.lsek_grouped_gemm_nvfp4(ptr(d), ptr(a), ptr(asf), ptr(w), ptr(tiles), ptr(d_off), None, None,
+                                     3, 40, 64, 128, None, ctypes.c_size_t(0),
+                                     ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert st == 0
+    sync_and_check_device_error()
+    assert (d == 3.0).all()
+
+
+def test_products_past_32_bits():
+    """An output of more than 2^31 elements, and a quantised tensor of as many:
+    the last rows are those of a small call on them alone."""
+    P = pk()
+    gen = torch.Generator().manual_seed(21)
+    n, k, rows = 7168, 64, 300_000
+    w, wsf, _ = rand_fp4(gen, 1, n, k)
+    tiles = P.nvfp4_tile_scales(wsf)
+    a = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda")
+    asf = torch.ones(rows, k // 16, device="cuda").to(torch.float8_e4m3fn)
+    out = P.grouped_gemm_nvfp4(a, asf, w, tiles, torch.tensor([0, rows], dtype=torch.int32, device="cuda"))
+    assert out.numel() > 2 ** 31
+    small = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
+    for at in (0, 299_593 - 100, rows - 100):  # 299593 rows hold 2^31 elements
+        want = P.grouped_gemm_nvfp4(a[at:at + 100].contiguous(), asf[at:at + 100].contiguous(), w, tiles, small)
+        assert torch.equal(out[at:at + 100], want)
+    codes, scales = P.nvfp4_quantize(out)
+    back = P.nvfp4_dequantize(codes, scales)
+    for at in (0, 299_593 - 100, rows - 100):
+        c, s = P.nvfp4_quantize(out[at:at + 100].contiguous())
+        assert torch.equal(codes[at:at + 100], c)
+        assert torch.equal(back[at:at + 100], P.nvfp4_dequantize(c, s))
+    sync_and_check_device_error()
+
+
+def test_two_products_on_two_streams():
+    """Two calls at once, each with its own stream and outputs, give what they
+    give alone."""
+    P = pk()
+    cases = [make_product([400, 3, 250], 512, 1024, seed=31), make_product([30] * 40, 288, 576, seed=32)]
+    want = [P.grouped_gemm_nvfp4(c[0], c[1], c[3], c[4], c[7]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (c, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(P.grouped_gemm_nvfp4(c[0], c[1], c[3], c[4], c[7]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
+    sync_and_check_device_error()
+
+
+def test_refusals_on_the_gpu():
+    """Types, shapes and places that the binding turns down before a launch."""
+    P = pk()
+    f8 = torch.float8_e4m3fn
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    codes, scales = P.nvfp4_quantize(x)
+    bad_calls = [
+        lambda: P.nvfp4_quantize(x.float()),
+        lambda: P.nvfp4_quantize(x[:, :24].contiguous()),
+        lambda: P.nvfp4_quantize(x.t()),
+        lambda: P.nvfp4_quantize(x, torch.ones(2, device="cuda")),
+        lambda: P.nvfp4_quantize(x, torch.ones(1)),
+        lambda: P.nvfp4_quantize(x, torch.ones(1, dtype=torch.float64, device="cuda")),
+        lambda: P.nvfp4_quantize(x[0]),
+        lambda: P.nvfp4_dequantize(codes, scales[:, :2].contiguous()),
+        lambda: P.nvfp4_dequantize(codes, scales.float()),
+        lambda: P.nvfp4_dequantize(codes, scales, dtype=torch.float64),
+        lambda: P.moe_permute_nvfp4(x.half(), torch.zeros(4, 2, dtype=torch.int32, device="cuda"), 4),
+        lambda: P.moe_permute_nvfp4(x, torch.zeros(4, 2, dtype=torch.int64, device="cuda"), 4),
+        lambda: P.moe_permute_nvfp4(x, torch.zeros(3, 2, dtype=torch.int32, device="cuda"), 4),
+        lambda: P.moe_permute_nvfp4(x, torch.zeros(4, 2, dtype=torch.int32, device="cuda"), 1024),
+    ]
+    w = torch.zeros(2, 128, 32, dtype=torch.uint8, device="cuda")
+    raw = torch.zeros(2, 128, 4, device="cuda").to(f8)
+    tiles = P.nvfp4_tile_scales(raw)
+    off = torch.tensor([0, 1, 4], dtype=torch.int32, device="cuda")
+    ok = (codes, scales, w, tiles, off)
+
+    def swap(i, t):
+        return lambda: P.grouped_gemm_nvfp4(*(t if j == i else v for j, v in enumerate(ok)))
+
+    bad_calls += [
+        swap(0, codes[:, :16].contiguous()), swap(0, x), swap(1, scales.float()), swap(2, w[:, :, :16].contiguous()),
+        swap(2, w[0]), swap(3, raw), swap(3, tiles[:1].contiguous()), swap(4, off[:2].contiguous()),
+        swap(4, off.long()), swap(4, off.cpu()),
+        lambda: P.grouped_gemm_nvfp4(*ok, torch.ones(2, device="cuda")),
+        lambda: P.grouped_gemm_nvfp4(*ok, None, torch.ones(1, device="cuda")),
+        lambda: P.grouped_gemm_swiglu_nvfp4(*ok),  # one part where two are due
+    ]
+    for i, call in enumerate(bad_calls):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+            raise AssertionError(f"call {i} was taken")
+    with pytest.raises(ValueError):  # swiglu_limit < 0, from the library
+        P.grouped_gemm_swiglu_nvfp4(codes, scales, w, P.nvfp4_tile_scales(raw, 2), off, swiglu_limit=-1.0)
+    assert P.grouped_gemm_nvfp4(*ok).shape == (4, 128)
 
 
 # ---- the layer --------------------------------------------------------------------

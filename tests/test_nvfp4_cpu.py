@@ -67,7 +67,7 @@ def test_product_refusals(lib):
     assert call(E=1024, N=1 << 21) == BAD       # weight rows past int32
     for name in ("D", "A", "sa", "B", "sb"):
         assert call(**{name: None}) == BAD
-        assert call(**{name: odd}) == BAD
+        assert call(**{name: ctypes.c_void_p(258) if name == "sa" else odd}) == BAD
     assert call(off=None) == BAD
     assert call(ws=ctypes.c_void_p(257)) == BAD
     assert call(rows=0, D=None, A=None) == 0
