@@ -567,8 +567,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kSfLoadWarp) {
     // ===================== TMA producer of scales =====================
-    // Runs up to kSfStages stages ahead of the scale warps, which release a slot as
-    // soon as they have read it, so scales wait in TMEM before their codes land.
+    // Runs up to kSfStages stages ahead of the scale warps, so that scales wait in
+    // TMEM before their codes land.
     if (elect_one()) {
       const uint64_t policy = policy_evict_last();
       bool ok = true;
@@ -742,8 +742,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int q = 0; q < 4 * kHalves; ++q)
             t[k * kSfTokCols + q] = q * 32 < kTok ? tok[q][k] : 0u;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.sf_empty_bar[slot]);
         // The MMAs of two stages before, which read this buffer, have completed.
         if (j >= 2)
           ok = __all_sync(0xffffffffu, wait_bar(&s.empty_bar[(j - 2) % kRecs], ((j - 2) / kRecs) & 1u,
@@ -755,8 +753,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st32(col + 2 * kSteps * 4, t);
         tmem_st_wait();
         tc_fence_before();
+        // The slot goes back only now that its bytes have gone through registers to
+        // TMEM, and with a proxy fence: these were ordinary loads, and the next
+        // bytes come through the async proxy, which overtakes a load that is still
+        // under way (a release right after the loads gave 1 % wrong outputs).
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.sf_bar[j & 1u]);
+        if (lane == 0) {
+          mbar_arrive(&s.sf_bar[j & 1u]);
+          mbar_arrive(&s.sf_empty_bar[slot]);
+        }
       }
     }
   } else {

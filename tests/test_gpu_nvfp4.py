@@ -225,6 +225,37 @@ def test_product_vs_64_bit_sum(counts, n, k):
     assert_product(out, av, wv, off, 0.75 * gb.astype(np.float64))
 
 
+@pytest.mark.parametrize("E,rows,n,k", [(8, 8192, 4096, 7168), (32, 6000, 2048, 768), (24, 7000, 3584, 2112)])
+def test_product_of_many_units_a_block(E, rows, n, k):
+    """Enough units that every block runs dozens of pipeline rounds at full load:
+    each ring slot is refilled many times while its last readers are busy.  Three
+    runs, each against the 64-bit sums, computed on the GPU."""
+    P = pk()
+    gen = torch.Generator(device="cuda").manual_seed(E)
+    cpu = torch.Generator().manual_seed(E)
+    counts = torch.bincount(torch.randint(0, E, (rows,), generator=cpu), minlength=E)
+    off = torch.zeros(E + 1, dtype=torch.int32)
+    off[1:] = counts.cumsum(0)
+    x = torch.randn(rows, k, device="cuda", generator=gen).to(torch.bfloat16)
+    w = (torch.randn(E, n, k, device="cuda", generator=gen) * 0.02).to(torch.bfloat16)
+    ga = glob(0.011)
+    a, asf = P.nvfp4_quantize(x, ga)
+    wc, wt, gw = P.nvfp4_quantize_weights(w)
+    av = P.nvfp4_dequantize(a, asf, None, torch.float32).double()  # code * scale, exact
+    wv = P.nvfp4_dequantize(wc, P.nvfp4_quantize(w, gw)[1], None, torch.float32)
+    outs = [P.grouped_gemm_nvfp4(a, asf, wc, wt, off.cuda(), ga, gw) for _ in range(3)]
+    sync_and_check_device_error()
+    for e in range(E):
+        lo, hi = int(off[e]), int(off[e + 1])
+        we, alpha = wv[e].double(), ga.double() * gw[e].double()
+        exact, mag = alpha * (av[lo:hi] @ we.T), alpha * (av[lo:hi].abs() @ we.abs().T)
+        acc = (k / 64 + 8 + 2) * 2.0 ** -23 * mag
+        bound = acc + 2.0 ** -8 * (exact.abs() + acc)
+        for out in outs:
+            over = ((out[lo:hi].double() - exact).abs() - bound).max()
+            assert over <= 0, f"expert {e}: {float(over):.3e} over the bound"
+
+
 @pytest.mark.parametrize("rows", [1, 24, 100, 150, 230])
 def test_product_exact_where_sums_are_exact(rows):
     """Scales that are powers of two: every partial sum is a multiple of 2^-6
