@@ -2,8 +2,8 @@
 
 A from-scratch implementation of the MoE-layer hot path of
 kkontosis/LayerStoRmExpertKernels: grouped top-k gating, permute/unpermute,
-fused SwiGLU, the bf16 expert gate/up/down contraction (tcgen05/TMEM/TMA) and
-the weighted (expert-parallel) combine.  The kernels live in liblsek.so behind
+fused SwiGLU, the bf16 and NVFP4 expert gate/up/down contractions
+(tcgen05/TMEM/TMA) and the weighted (expert-parallel) combine.  The kernels live in liblsek.so behind
 the C ABI of include/lsek.h; `_C` is the torch binding that exposes the
 reference's operator surface (csrc/bindings_python.cu:371-417 of the
 reference) under the same names.  `import sm120_expert_kernels` gives the same

@@ -13,10 +13,10 @@
 // nvfp4_quantize in a row, without their passes over memory.
 //
 // Tiling.  The weights are the MMA's M operand (two boxes of 128 rows), the
-// tokens its N operand (up to kTokRows, rounded up to 16): a tile's cost then
+// tokens its N operand (up to kTok, rounded up to 16): a tile's cost then
 // follows its token count, and a weight row passes through shared memory once
 // for every chunk of tokens.  An expert's rows are cut into equal chunks of at
-// most kTokRows.  Units are (expert, n-tile, chunk), chunk fastest, so chunks
+// most kTok.  Units are (expert, n-tile, chunk), chunk fastest, so chunks
 // that share a weight tile are taken at about the same time by neighbouring
 // CTAs and the weight tile comes from HBM once.  A persistent grid of one CTA
 // per SM: CTA i starts with unit i and takes its further ones from an atomic
@@ -33,10 +33,17 @@
 // that start at any expert boundary, from there too where TMA can load them
 // (K % 256 == 0: rows of whole 16-byte pieces) and from global memory
 // otherwise.  (Loading them from global memory always costs 45 to 70 % more
-// time at 128 to 1024 rows an expert: 32 lines a load, in four warps.)  Copying the same tiles
-// with tcgen05.cp takes the tensor pipe about 165 cycles for each 512 bytes, 12
-// to 16 of them a stage, in line with the MMAs: 1.5 times the whole kernel's
-// time (64 experts, H=7168, I=2048: 270 against 183 us at one row an expert).
+// time at 128 to 1024 rows an expert: 32 lines a load, in four warps.)  Copying
+// the weights' tiles with tcgen05.cp from the MMA warp instead is 1 to 9 % slower
+// (down product, 16 experts of 1024 rows: 171 against 156 us): eight more
+// instructions a stage in the lane that paces the MMAs.
+//
+// Bounds, measured on a B200 with 64 experts, H=7168, I=2048 (6.54 TB/s copy):
+// up to 64 rows an expert the weights' stream, gate/up 163 to 167 us = 6.5 to 6.3
+// TB/s; at 128 rows 190 us = 5.6 TB/s, where a tile takes both accumulators and
+// its epilogue's first part stands between two main loops; at 1024 rows (16
+// experts) 241 us = 4.0 PFLOP/s, bound by the loads into shared memory (64 KB a
+// stage of about 900 cycles) and that same gap.
 //
 // One CTA = 16 warps:
 //   warp 0       takes units; TMA producer of the weights' codes
@@ -46,7 +53,7 @@
 //                chunks of 16 tokens).  A chunk comes out of TMEM as bf16 pairs
 //                of the two boxes (g and u, or columns c and c + 128), the next
 //                one's load under its arithmetic.  bf16 outputs go straight to
-//                memory (64 bytes of a token a store); for NVFP4 outputs the
+//                memory, 4 bytes a lane after neighbours have traded; for NVFP4 outputs the
 //                warp turns its 16 x 32 piece in shared memory, so that a lane
 //                holds one block of 16 outputs of a token
 //   warps 10-13  scales: shared memory -> TMEM

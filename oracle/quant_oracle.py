@@ -3,8 +3,8 @@
 TEST INFRASTRUCTURE ONLY.  Only tests/ may import this module; nothing in the
 product does.  It restates, in numpy, the reference's CPU definitions of the
 quantised formats that its expert GEMMs take (kkontosis/LayerStoRmExpertKernels,
-tests/test_reference.py:19-107), the next row of the hot-path scope after the
-bf16 layer:
+tests/test_reference.py:19-107), and the definition of this library's NVFP4
+quantiser:
 
   * FP8 E4M3 with one float32 scale per 128 consecutive elements of a row
     (`ref_fp8_dequant`, test_reference.py:56-73; `ref_dynamic_fp8_quant`,
