@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t at = SWIGLU ? ((row0 + tok) * p.n_out + col0 + feat) / kFp4Block
                           : (row0 + (lane & 1)) * p.n_out + col0 + q * 32 + (lane & ~1);
       const uint32_t trade = (lane & 1) == 0 ? 0x5410u : 0x3276u;
-      const int64_t at_step = SWIGLU ? 2 * p.n_out : 32ll * p.n_out;  // 32 rows on
+      const int64_t at_step = SWIGLU ? 2ll * p.n_out : 32ll * p.n_out;  // 32 rows on
       const bool in0 = (SWIGLU ? feat : q * 32 + lane) < cols, in1 = kBoxRows + q * 32 + lane < cols;
 #pragma unroll 1
       for (int t0 = grp * 16; t0 < nn; t0 += 32, at += at_step) {
@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t o0 = __shfl_xor_sync(0xffffffffu, p0[i], 1);
             const uint32_t o1 = __shfl_xor_sync(0xffffffffu, p1[i], 1);
             if (t0 + 2 * i + (lane & 1) < u.rows) {
-              __nv_bfloat16* dst = p.D + at + 2 * i * p.n_out;
+              __nv_bfloat16* dst = p.D + at + 2ll * i * p.n_out;
               if (in0) *reinterpret_cast<uint32_t*>(dst) = __byte_perm(p0[i], o0, trade);
               if (in1) *reinterpret_cast<uint32_t*>(dst + kBoxRows) = __byte_perm(p1[i], o1, trade);
             }

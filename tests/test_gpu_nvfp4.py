@@ -509,6 +509,31 @@ def test_products_past_32_bits():
     sync_and_check_device_error()
 
 
+def test_product_wider_than_2_31_elements_in_16_rows():
+    """16 rows of 160 million columns: the rows of one 16-row chunk lie more than
+    2^31 elements apart (14 * N > 2^31).  The whole output equals products with
+    eight slices of the weights, each narrow enough for 32-bit offsets."""
+    P = pk()
+    n, k, rows, parts = 160_000_000, 64, 16, 8
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    a = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    asf = torch.exp2(torch.randint(-2, 3, (rows, k // 16), device="cuda", generator=gen).float()).to(torch.float8_e4m3fn)
+    w = torch.randint(0, 256, (1, n, k // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    # n is a multiple of 128, so any bytes are tiles of scales: E4M3 codes of 0.25 to 1.875
+    tiles = torch.randint(0x28, 0x40, (1, n // 128, k // 64, 512), dtype=torch.uint8, device="cuda",
+                          generator=gen).view(torch.float8_e4m3fn)
+    off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    out = P.grouped_gemm_nvfp4(a, asf, w, tiles, off)
+    sync_and_check_device_error()
+    step = n // parts
+    assert step % 128 == 0 and 14 * n > 2 ** 31 and 16 * step < 2 ** 31
+    for i in range(parts):
+        part = P.grouped_gemm_nvfp4(a, asf, w[:, i * step:(i + 1) * step],
+                                    tiles[:, i * step // 128:(i + 1) * step // 128], off)
+        assert torch.equal(out[:, i * step:(i + 1) * step], part), i
+    sync_and_check_device_error()
+
+
 def test_two_products_on_two_streams():
     """Two calls at once, each with its own stream and outputs, give what they
     give alone."""
