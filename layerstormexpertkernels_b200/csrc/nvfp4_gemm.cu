@@ -605,8 +605,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint64_t* full = &s.sf_full_bar[slot];
           const uint32_t bytes = min(kSteps, p.steps - kb * kSteps) * kSfTile;
           mbar_expect_tx(full, boxes * bytes + (p.sf_by_tma ? nn * 16 : 0));
-          bulk_load(st, sf + kb * kSfBoxBytes, bytes, full);
-          if (boxes == 2) bulk_load(st + kSfBoxBytes, sf2 + kb * kSfBoxBytes, bytes, full);
+          const int64_t at = static_cast<int64_t>(kb) * kSfBoxBytes;  // 8 K bytes a tile: past 2^31 in a long row
+          bulk_load(st, sf + at, bytes, full);
+          if (boxes == 2) bulk_load(st + kSfBoxBytes, sf2 + at, bytes, full);
           if (p.sf_by_tma) {
             for (int r = 0; r < nn;) {
               const int i = box_of(nn - r);

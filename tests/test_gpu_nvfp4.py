@@ -534,6 +534,36 @@ def test_product_wider_than_2_31_elements_in_16_rows():
     sync_and_check_device_error()
 
 
+def test_product_with_2_gb_of_scales_a_tile():
+    """K = 2^28 + 1024: a weight tile's scales take more than 2^31 bytes.  All
+    codes but the last 2048 of a row are zeros, so the output is that of a
+    product over the last 2048 alone."""
+    P = pk()
+    k, tail, n, rows = 2 ** 28 + 1024, 2048, 160, 3
+    gen = torch.Generator(device="cuda").manual_seed(43)
+
+    def ends(*shape):  # codes that are zeros but for the last `tail` of a row
+        t = torch.zeros(*shape, k // 2, dtype=torch.uint8, device="cuda")
+        t[..., -tail // 2:] = torch.randint(0, 256, (*shape, tail // 2), dtype=torch.uint8, device="cuda", generator=gen)
+        return t
+
+    a, w = ends(rows), ends(1, n)
+    asf = torch.ones(rows, k // 16, device="cuda").to(torch.float8_e4m3fn)
+    tiles = torch.full((1, 2, k // 64, 512), 0x38, dtype=torch.uint8, device="cuda")  # E4M3 1.0
+    last = torch.randint(0x28, 0x40, (1, 2, tail // 64, 512), dtype=torch.uint8, device="cuda", generator=gen)
+    tiles[:, :, -tail // 64:] = last
+    f8 = torch.float8_e4m3fn
+    off = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    assert tiles[0, 0].numel() > 2 ** 31
+    got = P.grouped_gemm_nvfp4(a, asf, w, tiles.view(f8), off)
+    sync_and_check_device_error()
+    want = P.grouped_gemm_nvfp4(a[:, -tail // 2:].contiguous(), asf[:, -tail // 16:].contiguous(),
+                                w[:, :, -tail // 2:].contiguous(), last.view(f8), off)
+    sync_and_check_device_error()
+    assert want.abs().sum() > 0
+    assert torch.equal(got, want)
+
+
 def test_two_products_on_two_streams():
     """Two calls at once, each with its own stream and outputs, give what they
     give alone."""
