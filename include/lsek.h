@@ -182,7 +182,10 @@ LSEK_API lsek_status lsek_moe_permute_noalloc(void* permuted_input, int32_t* exp
 /* Weighted unpermute.  fp32_output == 0: out [T,H] (dtype) =
  * round(sum_k fma(w[t,k], x[s2d[t,k]], acc)), fp32 accumulation in slot order.
  * fp32_output != 0: out is f32 [T,topk,H], out[t,k,:] = w[t,k]*x[s2d[t,k]]
- * (no cross-slot sum).  topk <= 32.  Replaces launch_moe_unpermute
+ * (no cross-slot sum).  A slot of weight 0 adds +0 whatever its row holds: the
+ * row of a pruned slot (index -1, weight 0) lies behind the last expert, where
+ * the grouped GEMMs write nothing.  The per-slot form below and the combine
+ * steps of lsek_ep_* follow the same rule.  topk <= 32.  Replaces launch_moe_unpermute
  * (smxx/permute/moe_permute.h:79-89, moe_permute.cu:602-642). */
 LSEK_API lsek_status lsek_moe_unpermute(void* output, const void* permuted_output,
                                const float* topk_weights,

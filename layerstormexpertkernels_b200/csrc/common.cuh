@@ -90,6 +90,14 @@ template <> struct Elem<__half> {
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 };
 
+// A slot's weighted value, rounded once.  A slot of weight 0 adds nothing,
+// whatever its row holds: a slot that adaptive gating pruned (index -1, weight
+// 0) has its row behind the last expert, which no product writes, and 0 times
+// what memory holds there may be NaN.
+__device__ __forceinline__ float weigh(float w, float x) {
+  return w == 0.0f ? 0.0f : __fmul_rn(w, x);
+}
+
 // Eight 16-bit elements in one 16-byte vector.
 template <typename T>
 struct alignas(16) Vec8 {

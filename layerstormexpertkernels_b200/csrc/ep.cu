@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) ep_combine_pack_kernel(
     uint4 out;
     __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(&out);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) o[q] = __float2bfloat16_rn(__fmul_rn(wk, __bfloat162float(e[q])));
+    for (int q = 0; q < 8; ++q) o[q] = __float2bfloat16_rn(weigh(wk, __bfloat162float(e[q])));
     *reinterpret_cast<uint4*>(dst + v * 8) = out;
   }
 }
@@ -493,7 +493,7 @@ __device__ __forceinline__ void push_combine_row(const PeerTable& peers, size_t 
       uint4 out;
       __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(&out);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) o[q] = __float2bfloat16_rn(__fmul_rn(wt, __bfloat162float(e[q])));
+      for (int q = 0; q < 8; ++q) o[q] = __float2bfloat16_rn(weigh(wt, __bfloat162float(e[q])));
       *reinterpret_cast<uint4*>(dst + v * 8) = out;
     }
   }

@@ -767,10 +767,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     static_cast<int64_t>(dr) * p.ldd + col0;
                 const float wt = __ldg(p.dst_w + pr);
                 if (w < cols_here)
-                  dst[w] = __float2bfloat16_rn(__fmul_rn(wt, round_bf16(__uint_as_float(v0[i]))));
+                  dst[w] = __float2bfloat16_rn(weigh(wt, round_bf16(__uint_as_float(v0[i]))));
                 if (kBoxRows + w < cols_here)
                   dst[kBoxRows + w] =
-                      __float2bfloat16_rn(__fmul_rn(wt, round_bf16(__uint_as_float(v1[i]))));
+                      __float2bfloat16_rn(weigh(wt, round_bf16(__uint_as_float(v1[i]))));
                 continue;
               }
               __nv_bfloat16* dst = dcol + static_cast<int64_t>(t) * p.ldd;
@@ -822,8 +822,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (COMBINE) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                  packed[j] = pack_bf16x2(__fmul_rn(wrow, round_bf16(__uint_as_float(v[2 * j]))),
-                                          __fmul_rn(wrow, round_bf16(__uint_as_float(v[2 * j + 1]))));
+                  packed[j] = pack_bf16x2(weigh(wrow, round_bf16(__uint_as_float(v[2 * j]))),
+                                          weigh(wrow, round_bf16(__uint_as_float(v[2 * j + 1]))));
               } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j)

@@ -508,13 +508,16 @@ __global__ void permute_rows_u16_kernel(const uint16_t* __restrict__ src, uint16
 
 constexpr int kUnpThreads = 128;
 
-// Loads the token's (dest row, weight) pairs into shared memory.
+// Loads the token's (dest row, weight) pairs into shared memory; the row of a
+// slot of weight 0, which is not to be read (see weigh() in common.cuh), is -1.
 __device__ __forceinline__ void load_slots(const float* __restrict__ w, const int32_t* __restrict__ s2d,
                                            int t, int topk, float* s_w, int32_t* s_d) {
   if (threadIdx.x < topk) {
     const int64_t i = static_cast<int64_t>(t) * topk + threadIdx.x;
-    s_w[threadIdx.x] = __ldg(w + i);
-    s_d[threadIdx.x] = __ldg(s2d + i);
+    const float wk = __ldg(w + i);
+    const int32_t d = __ldg(s2d + i);
+    s_w[threadIdx.x] = wk;
+    s_d[threadIdx.x] = wk == 0.0f ? -1 : d;
   }
   __syncthreads();
 }
@@ -550,7 +553,9 @@ __global__ void __launch_bounds__(kUnpThreads) unpermute_sum_kernel(
     uint4 raw[KMAX];
 #pragma unroll
     for (int k = 0; k < KMAX; ++k)
-      if (k < topk) raw[k] = ldg_nc_v4(in + static_cast<int64_t>(s_d[k]) * H + v * 8);
+      if (k < topk)
+        raw[k] = s_d[k] >= 0 ? ldg_nc_v4(in + static_cast<int64_t>(s_d[k]) * H + v * 8)
+                             : make_uint4(0, 0, 0, 0);
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < KMAX; ++k) {
@@ -578,7 +583,8 @@ __global__ void unpermute_sum_scalar_kernel(T* __restrict__ out, const T* __rest
   for (int h = threadIdx.x; h < H; h += blockDim.x) {
     float acc = 0.0f;
     for (int k = 0; k < topk; ++k)
-      acc = __fmaf_rn(s_w[k], Elem<T>::to_f(in[static_cast<int64_t>(s_d[k]) * H + h]), acc);
+      if (s_d[k] >= 0)
+        acc = __fmaf_rn(s_w[k], Elem<T>::to_f(in[static_cast<int64_t>(s_d[k]) * H + h]), acc);
     out[static_cast<int64_t>(t) * H + h] = Elem<T>::from_f(acc);
   }
 }
@@ -597,7 +603,7 @@ __global__ void __launch_bounds__(kUnpThreads) unpermute_perslot_kernel(
       float x[8];
       unpack8<T>(ldg_nc_v4(row + v * 8), x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(wk, x[j]);
+      for (int j = 0; j < 8; ++j) x[j] = weigh(wk, x[j]);
       if (OUT_F32) {
         float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + slot * H + v * 8);
         o[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -608,7 +614,7 @@ __global__ void __launch_bounds__(kUnpThreads) unpermute_perslot_kernel(
     }
   } else {
     for (int h = threadIdx.x; h < H; h += kUnpThreads) {
-      const float v = __fmul_rn(wk, Elem<T>::to_f(row[h]));
+      const float v = weigh(wk, Elem<T>::to_f(row[h]));
       if (OUT_F32) static_cast<float*>(out)[slot * H + h] = v;
       else static_cast<T*>(out)[slot * H + h] = Elem<T>::from_f(v);
     }

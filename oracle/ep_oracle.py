@@ -105,7 +105,8 @@ def ep_combine_pack(expert_out, s2d, ids, weights, slot_row) -> np.ndarray:
         for j in range(k):
             if ids[i, j] < 0:
                 continue
-            comb[q] = mo.bf16_round((w[i, j] * y[d[i, j]]).astype(F32))
+            if w[i, j] != 0:
+                comb[q] = mo.bf16_round((w[i, j] * y[d[i, j]]).astype(F32))
             q += 1
     return comb
 

@@ -197,8 +197,8 @@ def _lib():
 def moe_unpermute(permuted_bits, topk_weights, s2d, num_tokens: int, topk: int,
                   fp16: bool = False) -> np.ndarray:
     """out[t] = round16(sum_k fma(w[t,k], x[s2d[t,k]], acc)) in slot order
-    (finalize_moe_routing_bf16, moe_permute.cu:182-246).  permuted_bits is
-    uint16 [rows, H]; returns uint16 [T, H]."""
+    (finalize_moe_routing_bf16, moe_permute.cu:182-246), over the slots whose
+    weight is not 0.  permuted_bits is uint16 [rows, H]; returns uint16 [T, H]."""
     x = np.ascontiguousarray(permuted_bits, dtype=np.uint16)
     w = np.ascontiguousarray(topk_weights, dtype=F32).reshape(-1)
     d = np.ascontiguousarray(s2d, dtype=np.int32).reshape(-1)
@@ -211,11 +211,13 @@ def moe_unpermute(permuted_bits, topk_weights, s2d, num_tokens: int, topk: int,
 
 def moe_unpermute_perslot_f32(permuted, topk_weights, s2d, num_tokens: int, topk: int):
     """out[t,k,:] = w[t,k] * x[s2d[t,k]] in fp32, no cross-slot sum
-    (moe_permute.cu:330-376; tests/test_kernels.py:113-120)."""
+    (moe_permute.cu:330-376; tests/test_kernels.py:113-120); 0 where w is 0,
+    as the row of a pruned slot may hold anything."""
     x = np.asarray(permuted, dtype=F32)
     w = np.asarray(topk_weights, dtype=F32).reshape(num_tokens, topk)
     d = np.asarray(s2d).reshape(num_tokens, topk).astype(np.int64)
-    return (w[:, :, None] * x[d]).astype(F32)
+    with np.errstate(invalid="ignore"):
+        return np.where(w[:, :, None] == 0, F32(0), (w[:, :, None] * x[d]).astype(F32))
 
 
 def moe_unpermute_perslot_bf16(permuted, topk_weights, s2d, num_tokens: int, topk: int):

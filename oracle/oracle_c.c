@@ -57,6 +57,7 @@ void oracle_unpermute_sum(const uint16_t* in, const float* w, const int32_t* s2d
     for (int64_t h = 0; h < H; ++h) acc[h] = 0.0f;
     for (int32_t k = 0; k < K; ++k) {
       const float wk = w[t * K + k];
+      if (wk == 0.0f) continue; /* a pruned slot: its row may hold anything */
       const uint16_t* row = in + (int64_t)s2d[t * K + k] * H;
       if (is_fp16) {
         for (int64_t h = 0; h < H; ++h) acc[h] = fmaf(wk, f16_to_f32(row[h]), acc[h]);

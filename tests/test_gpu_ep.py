@@ -228,6 +228,33 @@ def test_ep_layer_peer_domain_one_rank(tokens, combine):
         assert dom.epoch == 3
 
 
+@pytest.mark.parametrize("tokens", [150, 1])
+@pytest.mark.parametrize("combine", ["fused", "push", "nccl"])
+def test_ep_layer_slot_of_weight_zero(tokens, combine):
+    """An expert that every token takes with weight 0 (its score underflows, its
+    bias selects it) and whose outputs are NaN adds nothing, in the combine of
+    each transport as in the canonical path."""
+    from layerstormexpertkernels_b200.ep import EPMoELayer, PeerDomain
+    w_gu, w_down, toks = _layer_setup(1, [tokens])
+    w_down = w_down.clone()
+    w_down[3] = float("nan")
+    x = toks[0]
+    x.logits[:, 3] = -200.0
+    bias = x.bias.clone()
+    bias[3] = 10.0
+    bias = bias.cuda()
+    ref = canonical_gpu(x, w_gu, w_down, bias)
+    assert not ref.isnan().any()
+    hidden, logits = x.hidden.cuda(), x.logits.cuda()
+    if combine == "nccl":
+        out = EPMoELayer(w_gu, w_down, bias, E_L, topk=K_L)(hidden, logits)
+    else:
+        with PeerDomain(max_tokens=512, hidden_dim=H_L, topk=K_L) as dom:
+            out = EPMoELayer(w_gu, w_down, bias, E_L, topk=K_L, domain=dom, combine=combine)(hidden, logits)
+            sync_and_check_device_error()
+    assert torch.equal(out.view(torch.int16), ref.view(torch.int16))
+
+
 def test_peer_combine_push_one_rank():
     """Dispatch + combine without a GEMM (synthetic expert outputs, as the
     EP combine benchmark runs it) against the canonical per-slot combine."""

@@ -630,6 +630,47 @@ def test_refusals_on_the_gpu():
     assert P.grouped_gemm_nvfp4(*ok).shape == (4, 128)
 
 
+@pytest.mark.parametrize("T,E,H,I,k,threshold", [(1, 8, 256, 64, 4, 0.5), (60, 16, 512, 128, 8, 0.6),
+                                                 (300, 8, 320, 192, 2, 0.7)])
+def test_chain_with_pruned_slots(T, E, H, I, k, threshold):
+    """adaptive_gating -> moe_permute_nvfp4 -> gate/up -> down -> moe_unpermute,
+    with NaN in every row behind the last expert that an operator leaves
+    unwritten: a token is the sum over its kept slots (the first of a token is
+    always kept; token T // 2 loses that one too)."""
+    from oracle import moe_oracle as O
+    from gpu_util import bits
+    P = pk()
+    gen = torch.Generator().manual_seed(T + E)
+    x = torch.randn(T, H, generator=gen).to(torch.bfloat16).cuda()
+    w_gu = (torch.randn(E, 2 * I, H, generator=gen) / np.sqrt(H)).to(torch.bfloat16).cuda()
+    w_down = (torch.randn(E, H, I, generator=gen) / np.sqrt(I)).to(torch.bfloat16).cuda()
+    w, idx = P.topk_gating(torch.randn(T, E, generator=gen).cuda(), None, k, 1, 1, 2.5, True)
+    w, idx, kept = P.adaptive_gating(w, idx, threshold)
+    w[T // 2], idx[T // 2] = 0.0, -1
+    valid = int((idx >= 0).sum())
+    assert valid < T * k
+    gx, gh = glob(0.01), glob(0.004)
+    a, asf, off, s2d, _ = P.moe_permute_nvfp4(x, idx, E, gx)
+    assert int(off[E]) == valid
+    gu, gut, gug = P.nvfp4_quantize_weights(w_gu, 2)
+    dn, dnt, dng = P.nvfp4_quantize_weights(w_down, 1)
+    h, hs = P.grouped_gemm_swiglu_nvfp4(a, asf, gu, gut, off, gx, gug, gh)
+    h[valid:] = 0xFF
+    hs.view(torch.uint8)[valid:] = 0x7F  # NaN
+    y = P.grouped_gemm_nvfp4(h, hs, dn, dnt, off, gh, dng)
+    y[valid:] = float("nan")
+    assert not y[:valid].isnan().any()
+    out = P.moe_unpermute(y, w, s2d, T, k)
+    sync_and_check_device_error()
+    assert not out.isnan().any() and (out[T // 2] == 0).all()
+    zeros = torch.where(torch.arange(T * k, device="cuda")[:, None] < valid, y, 0)
+    assert np.array_equal(bits(out), O.moe_unpermute(bits(zeros), w.cpu().numpy(), s2d.cpu().numpy(), T, k))
+    slots = (zeros.double()[s2d.long()].view(T, k, H) * w.double()[..., None])
+    # k fp32 steps and one rounding to bf16
+    bound = slots.abs().sum(1) * k * 2.0 ** -24 + slots.sum(1).abs() * 2.0 ** -8 * (1 + 2.0 ** -10)
+    assert ((out.double() - slots.sum(1)).abs() <= bound).all()
+
+
 # ---- the layer --------------------------------------------------------------------
 
 

@@ -276,6 +276,34 @@ def test_reference_perslot_cases():
         assert torch.equal(ek().moe_combine_reduce_slots_bf16_to_bf16((a + b).contiguous()), out16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,k,H", [(1, 1, 8), (96, 8, 7168), (300, 6, 1000), (64, 3, 13), (5, 16, 256),
+                                   (9, 32, 64)])
+def test_unpermute_takes_nothing_from_slots_of_weight_zero(T, k, H, dtype):
+    """The rows of slots of weight 0 hold NaN, infinities and the largest
+    values, as memory that nothing wrote may; the other slots' sums have the
+    bits that they have with zeros there, and a token of such slots alone is 0."""
+    permuted, w, s2d = unpermute_inputs(T, k, H, seed=T + k + H, dtype=dtype)
+    g = torch.Generator().manual_seed(k)
+    gone = torch.rand(T, k, generator=g) < 0.3
+    gone[T // 2] = True
+    w[gone] = torch.where(torch.rand(int(gone.sum()), generator=g) < 0.5, 0.0, -0.0)
+    junk = torch.tensor([float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).max, -1.0], dtype=dtype)
+    clean, rows = permuted.clone(), s2d.view(T, k)[gone].long()
+    permuted[rows] = junk[torch.randint(0, 5, (rows.numel(), H), generator=g)]
+    clean[rows] = 0.0
+    pc, cc, wc, sc = permuted.cuda(), clean.cuda(), w.cuda(), s2d.cuda()
+    ops = [lambda x: ek().moe_unpermute(x, wc, sc, T, k), lambda x: ek().moe_unpermute_fp32(x, wc, sc, T, k)]
+    if dtype == torch.bfloat16:
+        ops.append(lambda x: ek().moe_unpermute_bf16_perslot(x, wc, sc, T, k))
+    for op in ops:
+        got, want = op(pc), op(cc)
+        assert torch.equal(got, want)
+        assert not want.isnan().any() and (got[T // 2] == 0).all()
+    ref = O.moe_unpermute(bits(permuted), w.numpy(), s2d.numpy(), T, k, fp16=dtype == torch.float16)
+    assert np.array_equal(bits(ops[0](pc)), ref)
+
+
 # ---- SwiGLU ----------------------------------------------------------------------------
 
 def check_swiglu(out, gate, up, limit):
