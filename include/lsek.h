@@ -222,7 +222,7 @@ LSEK_API lsek_status lsek_moe_combine_reduce_slots(void* output_bf16,
 
 /* Fused SwiGLU: out [N,d] = silu(g) * u with g = in[:, :d], u = in[:, d:],
  * computed in fp32, stored in dtype.  swiglu_limit > 0 clamps
- * g = min(g, L), u = clamp(u, -L, L) first.  Replaces launch_fused_swiglu
+ * g = min(g, L), u = clamp(u, -L, L) first; NaN stays NaN.  Replaces launch_fused_swiglu
  * (smxx/activation/fused_swiglu.h:22-27, fused_swiglu.cu:156-183). */
 LSEK_API lsek_status lsek_fused_swiglu(void* output, const void* input,
                               int32_t num_tokens, int32_t d,

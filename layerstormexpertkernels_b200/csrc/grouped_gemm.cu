@@ -688,6 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // time of one.
     const int q = warp & 3;           // TMEM lane quarter this warp may access
     const int grp = (warp - 2) >> 2;  // column half this warp drains
+    const float clamp = SWIGLU ? clamp_limit(p.swiglu_limit) : 0.0f;
     int qslot = 0;
     uint32_t qphase = 0;
     uint32_t ac = 0;
@@ -778,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (w < cols_here)
                   dst[w] = __float2bfloat16_rn(swiglu_f32(round_bf16(__uint_as_float(v0[i])),
                                                           round_bf16(__uint_as_float(v1[i])),
-                                                          p.swiglu_limit));
+                                                          clamp));
               } else {
                 if (w < cols_here) dst[w] = __float2bfloat16_rn(__uint_as_float(v0[i]));
                 if (kBoxRows + w < cols_here)
@@ -798,10 +799,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
                 const float h0 = swiglu_f32(round_bf16(__uint_as_float(g[2 * j])),
-                                            round_bf16(__uint_as_float(u[2 * j])), p.swiglu_limit);
+                                            round_bf16(__uint_as_float(u[2 * j])), clamp);
                 const float h1 = swiglu_f32(round_bf16(__uint_as_float(g[2 * j + 1])),
-                                            round_bf16(__uint_as_float(u[2 * j + 1])),
-                                            p.swiglu_limit);
+                                            round_bf16(__uint_as_float(u[2 * j + 1])), clamp);
                 packed[j] = pack_bf16x2(h0, h1);
               }
               uint4* dst = reinterpret_cast<uint4*>(drow + c);

@@ -324,8 +324,8 @@ __device__ __forceinline__ void swiglu_turn(const uint32_t (&g2)[8], const uint3
   for (int i = 0; i < 8; ++i) {
     float2 g = unpack2(g2[i], __nv_bfloat16()), u = unpack2(u2[i], __nv_bfloat16());
     if (CLAMP) {
-      g = make_float2(fminf(g.x, limit), fminf(g.y, limit));
-      u = make_float2(fminf(fmaxf(u.x, -limit), limit), fminf(fmaxf(u.y, -limit), limit));
+      g = make_float2(clamp_gate(g.x, limit), clamp_gate(g.y, limit));
+      u = make_float2(clamp_up(u.x, limit), clamp_up(u.y, limit));
     }
     const float2 t = mul_f32x2(g.x, g.y, -1.4426950408889634f, -1.4426950408889634f);
     float e0, e1, r0, r1;

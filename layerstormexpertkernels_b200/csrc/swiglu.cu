@@ -26,9 +26,21 @@ __global__ void __launch_bounds__(256) swiglu_vec_kernel(T* __restrict__ out,
     const T* ue = reinterpret_cast<const T*>(&uraw);
     uint4 oraw;
     T* oe = reinterpret_cast<T*>(&oraw);
+    float gf[8], uf[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      oe[j] = Elem<T>::from_f(swiglu_f32(Elem<T>::to_f(ge[j]), Elem<T>::to_f(ue[j]), limit));
+    for (int j = 0; j < 8; ++j) {
+      gf[j] = Elem<T>::to_f(ge[j]);
+      uf[j] = Elem<T>::to_f(ue[j]);
+    }
+    if (limit > 0.0f) {  // one branch for the eight
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        gf[j] = clamp_gate(gf[j], limit);
+        uf[j] = clamp_up(uf[j], limit);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) oe[j] = Elem<T>::from_f(silu_mul(gf[j], uf[j]));
     *reinterpret_cast<uint4*>(out + n * d + static_cast<int64_t>(v) * 8) = oraw;
   }
 }
@@ -37,13 +49,14 @@ template <typename T>
 __global__ void swiglu_scalar_kernel(T* __restrict__ out, const T* __restrict__ in, int64_t N,
                                      int d, float limit) {
   const int64_t total = N * d;
+  const float clamp = clamp_limit(limit);
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t n = i / d;
     const int j = static_cast<int>(i - n * d);
     const float g = Elem<T>::to_f(in[n * 2 * d + j]);
     const float u = Elem<T>::to_f(in[n * 2 * d + d + j]);
-    out[i] = Elem<T>::from_f(swiglu_f32(g, u, limit));
+    out[i] = Elem<T>::from_f(swiglu_f32(g, u, clamp));
   }
 }
 

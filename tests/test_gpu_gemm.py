@@ -111,6 +111,24 @@ def test_swiglu_epilogue_equals_unfused(counts, K, I, limit):
     assert_close_bf16(fused, ref)
 
 
+def test_swiglu_epilogue_clamp_keeps_nan():
+    """A NaN in a token makes its whole output row NaN under the clamp, in small
+    and in full tiles, and leaves the other rows as without it."""
+    a, w, off = make_problem([5, 0, 200, 130], 256, 256, seed=23, wscale=0.25)
+    a, w, off = a.cuda(), w.cuda(), off.cuda()
+    want = ek().grouped_gemm_swiglu_bf16(a, w, off, swiglu_limit=1.0)
+    bad = [2, 77, 204, 333]
+    a[bad, 9] = float("nan")
+    got = ek().grouped_gemm_swiglu_bf16(a, w, off, swiglu_limit=1.0)
+    unfused = ek().fused_swiglu(ek().grouped_gemm_bf16(a, w, off), swiglu_limit=1.0)
+    sync_and_check_device_error()
+    assert got[bad].isnan().all()
+    assert torch.equal(got.view(torch.int16), unfused.view(torch.int16))
+    rest = torch.ones(335, dtype=torch.bool)
+    rest[bad] = False
+    assert torch.equal(got[rest.cuda()], want[rest.cuda()])
+
+
 def test_deepseek_shape_subset():
     """Eight experts of the DeepSeek-V3 layer (H=7168, I=2048) with ~128 rows
     each: gate/up + SwiGLU then down, against the double-precision oracle."""

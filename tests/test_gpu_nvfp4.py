@@ -458,6 +458,37 @@ def test_swiglu_for_every_gate_value():
     sync_and_check_device_error()
 
 
+def test_swiglu_clamp_keeps_nan():
+    """A token with NaN among its values is NaN in every block behind the
+    clamped gate/up kernel and behind the layer, and the other tokens are as
+    without it; the plain product, fused_swiglu and the quantiser agree."""
+    P = pk()
+    layer, x, logits = make_layer(200, 8, 512, 192, 2, 1, 1, seed=17, limit=1.0)
+    want = layer(x, logits)
+    x[50, 7], x[120, 500], x[199, 0] = float("nan"), float("inf"), -float("inf")
+    bad = torch.zeros(200, dtype=torch.bool, device="cuda")
+    bad[[50, 120, 199]] = True
+    out = layer(x, logits)
+    assert out[bad].isnan().all()
+    assert not want.isnan().any() and torch.equal(out[~bad], want[~bad])
+    w, idx = P.topk_gating(logits, layer.bias, 2, 1, 1, 2.5, True)
+    a, asf, off, s2d, perm = P.moe_permute_nvfp4(x, idx, 8, layer.hidden_global_scale)
+    args = (off, layer.hidden_global_scale, layer.w_gu_global_scale)
+    h, hs = P.grouped_gemm_swiglu_nvfp4(a, asf, layer.w_gu, layer.w_gu_scales, *args,
+                                        layer.inter_global_scale, swiglu_limit=1.0)
+    rows = bad[perm.long() // 2]
+    assert (hs.view(torch.uint8)[rows] == 0x7F).all() and (hs.view(torch.uint8)[~rows] != 0x7F).all()
+    # the gate rows and the up rows apart, as the tiles hold them
+    half = layer.w_gu.shape[1] // 2
+    tall = layer.w_gu_scales.shape[1] // 2
+    gu = torch.cat([P.grouped_gemm_nvfp4(a, asf, layer.w_gu[:, i * half:(i + 1) * half].contiguous(),
+                                         layer.w_gu_scales[:, i * tall:(i + 1) * tall].contiguous(), *args)
+                    for i in range(2)], 1)
+    q, qs = P.nvfp4_quantize(P.fused_swiglu(gu, swiglu_limit=1.0), layer.inter_global_scale)
+    assert torch.equal(q, h) and torch.equal(qs.view(torch.uint8), hs.view(torch.uint8))
+    sync_and_check_device_error()
+
+
 def test_more_than_256_experts():
     P = pk()
     gen = torch.Generator().manual_seed(12)

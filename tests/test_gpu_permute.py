@@ -364,6 +364,27 @@ def test_swiglu_fp16():
     check_swiglu(out.cpu(), gate, up, 0.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,d", [(40, 256), (7, 13)])
+def test_swiglu_clamp_keeps_nan(N, d, dtype):
+    """NaN in the gate or the up half stays NaN under a clamp, at its own place
+    only, as torch.clamp keeps it; infinities are clamped."""
+    g = torch.Generator().manual_seed(d)
+    gate, up = (torch.randn(N, d, generator=g) * 4).to(dtype), (torch.randn(N, d, generator=g) * 4).to(dtype)
+    for i, t in enumerate((gate, up)):
+        t.view(-1)[torch.randperm(N * d, generator=g)[:9 + i]] = float("nan")
+    gate[1, 2], up[1, 2], gate[2, 3], up[2, 3] = float("inf"), -float("inf"), 1.0, float("inf")
+    nan = gate.isnan() | up.isnan()
+    for limit in (0.0, 2.0):
+        out = ek().fused_swiglu(torch.cat([gate, up], 1).cuda(), swiglu_limit=limit).cpu()
+        assert torch.equal(out.isnan(), nan)
+        ref = torch.as_tensor(O.swiglu(gate.float().numpy(), up.float().numpy(), limit)).double()
+        ok = ~nan & ref.isfinite()
+        assert torch.equal(out.isinf(), ref.isinf())
+        step = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -10
+        assert ((out.double() - ref).abs()[ok] <= ref.abs()[ok] * step + 2.0 ** -24).all()
+
+
 def test_reference_swiglu_cases():
     # tests/test_kernels.py:41-56, 318-336 and tests/test_fused_swiglu.py:127-201
     N, D = 256, 2048
