@@ -605,9 +605,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint64_t* full = &s.sf_full_bar[slot];
           const uint32_t bytes = min(kSteps, p.steps - kb * kSteps) * kSfTile;
           mbar_expect_tx(full, boxes * bytes + (p.sf_by_tma ? nn * 16 : 0));
-          const int64_t at = static_cast<int64_t>(kb) * kSfBoxBytes;  // 8 K bytes a tile: past 2^31 in a long row
-          bulk_load(st, sf + at, bytes, full);
-          if (boxes == 2) bulk_load(st + kSfBoxBytes, sf2 + at, bytes, full);
+          bulk_load(st, sf, bytes, full);
+          if (boxes == 2) bulk_load(st + kSfBoxBytes, sf2, bytes, full);
+          sf += kSfBoxBytes;  // a tile has 8 K bytes, more than an int in a long row
+          sf2 += kSfBoxBytes;
           if (p.sf_by_tma) {
             for (int r = 0; r < nn;) {
               const int i = box_of(nn - r);
@@ -833,6 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t at = SWIGLU ? ((row0 + tok) * p.n_out + col0 + feat) / kFp4Block
                           : (row0 + (lane & 1)) * p.n_out + col0 + q * 32 + (lane & ~1);
       const uint32_t trade = (lane & 1) == 0 ? 0x5410u : 0x3276u;
+      const int64_t pair_step = 2ll * p.n_out;
       const int64_t at_step = SWIGLU ? 2ll * p.n_out : 32ll * p.n_out;  // 32 rows on
       const bool in0 = (SWIGLU ? feat : q * 32 + lane) < cols, in1 = kBoxRows + q * 32 + lane < cols;
 #pragma unroll 1
@@ -861,12 +863,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           // Neighbouring lanes trade, so that an even lane has two columns of the
           // even token of a pair and an odd lane those of the odd one.
+          __nv_bfloat16* dst = p.D + at;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 8; ++i, dst += pair_step) {
             const uint32_t o0 = __shfl_xor_sync(0xffffffffu, p0[i], 1);
             const uint32_t o1 = __shfl_xor_sync(0xffffffffu, p1[i], 1);
             if (t0 + 2 * i + (lane & 1) < u.rows) {
-              __nv_bfloat16* dst = p.D + at + 2ll * i * p.n_out;
               if (in0) *reinterpret_cast<uint32_t*>(dst) = __byte_perm(p0[i], o0, trade);
               if (in1) *reinterpret_cast<uint32_t*>(dst + kBoxRows) = __byte_perm(p1[i], o1, trade);
             }
