@@ -66,12 +66,46 @@ class StageEvents:
             self.handles = []
 
 
-class MoELayer:
+class LayerWorkspace:
+    """The reusable workspace of a layer: it grows to the largest token count
+    seen.  A workspace that a captured graph writes at each replay is kept for
+    as long as the layer lives when a larger one takes its place; any other one
+    goes back to the allocator once the current stream has done with it (the
+    allocator by itself asks only for the stream that the memory came from).
+    """
+
+    def _init_workspace(self, device, max_tokens: int) -> None:
+        self._workspace_device = device
+        self._captured = False  # whether a capture has used self.workspace
+        self._kept = []         # outgrown workspaces of captured graphs
+        self.workspace = torch.empty(0, dtype=torch.uint8, device=device)
+        if max_tokens:
+            self._ensure_workspace(max_tokens)
+
+    def _ensure_workspace(self, num_tokens: int) -> None:
+        need = self.workspace_bytes(num_tokens)
+        if self.workspace.numel() < need:
+            if self._captured:
+                self._kept.append(self.workspace)
+            elif self.workspace.is_cuda:
+                self.workspace.record_stream(torch.cuda.current_stream(self.workspace.device))
+            self._captured = False
+            self.workspace = torch.empty(need, dtype=torch.uint8, device=self._workspace_device)
+        if not self._captured and self._capturing():
+            self._captured = True
+
+    def _capturing(self) -> bool:
+        return self.workspace.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+class MoELayer(LayerWorkspace):
     """A routed-expert layer with resident weights and a reusable workspace.
 
     The workspace grows to the largest token count seen and is reused, so a
     steady-state forward allocates only its output (or nothing, with `out=`),
-    which keeps the call capturable in a CUDA graph.
+    which keeps the call capturable in a CUDA graph.  Calls on different
+    streams, replays included, need a layer each: they would share the
+    workspace.
     """
 
     def __init__(self, w_gu: torch.Tensor, w_down: torch.Tensor,
@@ -90,18 +124,11 @@ class MoELayer:
         self.renormalize = renormalize
         self.scoring_func = scoring_func
         self.swiglu_limit = swiglu_limit
-        self.workspace = torch.empty(0, dtype=torch.uint8, device=w_gu.device)
-        if max_tokens:
-            self._ensure_workspace(max_tokens)
+        self._init_workspace(w_gu.device, max_tokens)
 
     def workspace_bytes(self, num_tokens: int) -> int:
         return _C.moe_layer_workspace_size(num_tokens, self.hidden_dim, self.inter_dim,
                                            self.num_experts, self.topk)
-
-    def _ensure_workspace(self, num_tokens: int) -> None:
-        need = self.workspace_bytes(num_tokens)
-        if self.workspace.numel() < need:
-            self.workspace = torch.empty(need, dtype=torch.uint8, device=self.w_gu.device)
 
     def forward(self, hidden: torch.Tensor, logits: torch.Tensor,
                 out: Optional[torch.Tensor] = None,

@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from . import _C
-from .layer import StageEvents
+from .layer import LayerWorkspace, StageEvents
 
 E2M1_MAX = 6.0
 E4M3_MAX = 448.0
@@ -100,7 +100,7 @@ def moe_layer_forward_nvfp4(hidden: torch.Tensor, logits: torch.Tensor,
     return out
 
 
-class MoELayerNVFP4:
+class MoELayerNVFP4(LayerWorkspace):
     """A routed-expert layer with resident NVFP4 weights and a reusable
     workspace: MoELayer's interface on 4-bit experts.
 
@@ -134,9 +134,7 @@ class MoELayerNVFP4:
         self.swiglu_limit = swiglu_limit
         self.hidden_global_scale = hidden_global_scale
         self.inter_global_scale = inter_global_scale
-        self.workspace = torch.empty(0, dtype=torch.uint8, device=w_gu.device)
-        if max_tokens:
-            self._ensure_workspace(max_tokens)
+        self._init_workspace(w_gu.device, max_tokens)
 
     @classmethod
     def from_weights(cls, w_gu: torch.Tensor, w_down: torch.Tensor,
@@ -149,11 +147,6 @@ class MoELayerNVFP4:
     def workspace_bytes(self, num_tokens: int) -> int:
         return _C.moe_layer_nvfp4_workspace_size(num_tokens, self.hidden_dim, self.inter_dim,
                                                  self.num_experts, self.topk)
-
-    def _ensure_workspace(self, num_tokens: int) -> None:
-        need = self.workspace_bytes(num_tokens)
-        if self.workspace.numel() < need:
-            self.workspace = torch.empty(need, dtype=torch.uint8, device=self.w_gu.device)
 
     def forward(self, hidden: torch.Tensor, logits: torch.Tensor,
                 out: Optional[torch.Tensor] = None,

@@ -815,3 +815,49 @@ def test_layer_stage_events_and_empty_batch():
     torch.cuda.synchronize()
     assert set(ev.elapsed_ms()) == set(P.STAGES)
     assert layer(x[:0], logits[:0]).shape == (0, 256)
+
+
+def test_replay_after_the_workspace_has_grown():
+    """A graph captured for few tokens is replayed after an eager call of many
+    has outgrown its workspace: the replay gives its bits and writes into no
+    memory that was handed out since."""
+    layer, x, logits = make_layer(500, 8, 512, 192, 2, 1, 1, seed=51)
+    few, few_logits, out = x[:6].contiguous(), logits[:6].contiguous(), torch.empty_like(x[:6])
+    layer(few, few_logits, out=out)
+    size = layer.workspace.numel()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        layer(few, few_logits, out=out)
+    want = by_operators(layer, few, few_logits)[0]
+    many = by_operators(layer, x, logits)[0]
+    assert torch.equal(layer(x, logits), many) and layer.workspace.numel() > size
+    taken = [torch.full((size,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(40)]
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert all((t == 0x5A).all() for t in taken)
+    assert torch.equal(layer(x, logits), many)
+    sync_and_check_device_error()
+
+
+def test_outgrown_workspace_waits_for_the_stream_that_uses_it():
+    """A workspace that came from the default stream and is outgrown on another
+    is handed out again only when that stream has done with it."""
+    layer, x, logits = make_layer(500, 8, 512, 192, 2, 1, 1, seed=52)
+    few, few_logits = x[:6].contiguous(), logits[:6].contiguous()
+    want, many = layer(few, few_logits), by_operators(layer, x, logits)[0]
+    old, size = layer.workspace.data_ptr(), layer.workspace.numel()
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        torch.cuda._sleep(400_000_000)  # some 0.2 s
+        a = layer(few, few_logits)
+        b = layer(x, logits)
+    taken = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(40)]
+    assert not st.query(), "the stream was done too early for the test to say anything"
+    assert all(t.data_ptr() != old for t in taken)
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, many)
+    sync_and_check_device_error()

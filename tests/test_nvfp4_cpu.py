@@ -120,6 +120,43 @@ def test_binding_rejects_cpu_tensors():
             f()
 
 
+@pytest.mark.parametrize("nvfp4", [False, True])
+def test_workspace_of_a_captured_graph_outlives_its_growth(nvfp4):
+    """A captured graph keeps writing to the workspace that it was captured
+    with, so that one stays allocated when a larger call outgrows it; one that
+    no capture used is let go."""
+    import weakref
+
+    u8, f8 = torch.uint8, torch.float8_e4m3fn
+    if nvfp4:
+        layer = P.MoELayerNVFP4(torch.zeros(4, 128, 64, dtype=u8), torch.zeros(4, 2, 2, 512).to(f8), None,
+                                torch.zeros(4, 128, 32, dtype=u8), torch.zeros(4, 1, 1, 512).to(f8), None, topk=2)
+    else:
+        layer = P.MoELayer(torch.zeros(4, 128, 64, dtype=torch.bfloat16),
+                           torch.zeros(4, 64, 64, dtype=torch.bfloat16), topk=2)
+    layer._ensure_workspace(4)
+    first = weakref.ref(layer.workspace)
+    layer._ensure_workspace(40)
+    assert first() is None and layer.workspace.numel() >= layer.workspace_bytes(40)
+    layer._capturing = lambda: True
+    layer._ensure_workspace(30)
+    captured = weakref.ref(layer.workspace)
+    layer._capturing = lambda: False
+    layer._ensure_workspace(4000)
+    later = weakref.ref(layer.workspace)
+    assert captured() is not None and captured() is not layer.workspace
+    layer._ensure_workspace(8000)
+    assert captured() is not None and later() is None
+    layer._capturing = lambda: True
+    layer._ensure_workspace(9000)  # grown inside a capture
+    inside = weakref.ref(layer.workspace)
+    layer._capturing = lambda: False
+    layer._ensure_workspace(10000)
+    assert inside() is not None and captured() is not None
+    del layer
+    assert captured() is None and inside() is None
+
+
 def test_tile_scales_places_every_scale():
     gen = torch.Generator().manual_seed(0)
     for e, n, s, parts in [(1, 32, 4, 1), (2, 300, 12, 1), (3, 320, 8, 2), (1, 256, 4, 2)]:
