@@ -288,7 +288,7 @@ LSEK_API lsek_status lsek_grouped_gemm_swiglu_bf16(void* Hout, const void* A,
  *   code  = e2m1(x * (1 / (scale * global_scale))) saturating at 6
  * (nearest, halves to even; codes 0 where the scale is 0).  A block that
  * holds an infinity or a NaN gets the scale NaN.  k % 16 == 0; global scales
- * are positive, in [2^-100, 2^100]; codes 8-byte aligned. */
+ * are positive, in [2^-100, 2^117]; codes 8-byte aligned. */
 LSEK_API lsek_status lsek_nvfp4_quantize(void* codes, void* scales, const void* x,
                                 const float* global_scale, int64_t groups, int64_t rows,
                                 int32_t k, int32_t dtype, void* stream);

@@ -16,7 +16,9 @@
 // the other by the rounding of inv, so an implementation with other steps
 // would give other codes.  A block that holds an infinity or a NaN gets the
 // scale NaN (0x7F) and codes of 0, so that it dequantises to NaN and is seen
-// downstream.  g has to be positive, in [2^-100, 2^100].
+// downstream.  g has to be positive, in [2^-100, 2^117]: s g and its reciprocal
+// are normal fp32 numbers there (s is 2^-9 to 448), and the largest bf16 tensor,
+// with g = amax / 2688, lies inside.
 #pragma once
 
 #include "common.cuh"

@@ -20,6 +20,7 @@ from .layer import LayerWorkspace, StageEvents
 
 E2M1_MAX = 6.0
 E4M3_MAX = 448.0
+MIN_GLOBAL_SCALE = 2.0 ** -100
 
 
 def nvfp4_tile_scales(scales: torch.Tensor, parts: int = 1) -> torch.Tensor:
@@ -46,16 +47,24 @@ def nvfp4_tile_scales(scales: torch.Tensor, parts: int = 1) -> torch.Tensor:
     return full.reshape(e, parts * tall, s // 4, 512).view(torch.float8_e4m3fn)
 
 
+def weight_global_scales(w: torch.Tensor) -> torch.Tensor:
+    """[E] float32 of weights [E, N, K]: see nvfp4_quantize_weights."""
+    if not w.numel():
+        return w.new_ones(w.shape[0], dtype=torch.float32)
+    amax = torch.stack([x.abs().nan_to_num_(0.0, posinf=0.0).amax() for x in w]).float()
+    return torch.where(amax > 0, (amax / (E2M1_MAX * E4M3_MAX)).clamp_(min=MIN_GLOBAL_SCALE), 1.0)
+
+
 def nvfp4_quantize_weights(w: torch.Tensor, parts: int = 1):
     """Expert weights [E, N, K] bf16 or fp16 -> (codes [E, N, K/2], tiled
     scales, global scales [E] float32).  An expert's global scale is its
-    largest magnitude / (6 * 448), which puts its largest block scale at the
-    top of E4M3 (1 for an expert of zeros)."""
+    largest finite magnitude / (6 * 448), which puts its largest block scale at
+    the top of E4M3 (1 for an expert of zeros, and never below 2^-100, the
+    least that the quantiser takes).  A block that holds an infinity or a NaN
+    gets the scale NaN; the expert's other blocks are as without it."""
     if w.dim() != 3:
         raise ValueError("nvfp4_quantize_weights: weights must be [E, N, K]")
-    glob = torch.stack([x.abs().amax() for x in w]).float() / (E2M1_MAX * E4M3_MAX) \
-        if w.numel() else w.new_ones(w.shape[0], dtype=torch.float32)
-    glob = torch.where(glob > 0, glob, 1.0)
+    glob = weight_global_scales(w)
     codes, scales = _C.nvfp4_quantize(w, glob)
     return codes, nvfp4_tile_scales(scales, parts), glob
 

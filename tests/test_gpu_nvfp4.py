@@ -160,6 +160,32 @@ def test_round_trip_is_near():
     assert (err <= amax * (1 / 6 + 2.0 ** -4) * (1 + 2.0 ** -20)).all()
 
 
+@pytest.mark.parametrize("exponent", [-131, -120, -105, -95, -60, 0, 60, 124])
+def test_quantize_weights_of_any_size(exponent):
+    """Weights from the smallest bf16 numbers to the largest come back within the
+    codes' and scales' steps (of the block, and of the smallest scale, 2^-9, where
+    the global scale is at its least), and a block with an infinity or a NaN is
+    NaN alone."""
+    P = pk()
+    gen = torch.Generator().manual_seed(exponent + 200)
+    w = torch.randn(3, 64, 256, generator=gen).clamp(-3.9, 3.9).to(torch.bfloat16)
+    w = (w.double() * 2.0 ** exponent).to(torch.bfloat16).cuda()
+    w[0, :, 32:48] = 0.0
+    w[1, 5, 3], w[2, 7, 100], w[2, 9, 255] = float("inf"), float("nan"), -float("inf")
+    codes, tiles, g = P.nvfp4_quantize_weights(w)
+    rows = P.nvfp4_quantize(w, g)
+    assert torch.equal(rows[0], codes)
+    assert torch.equal(P.nvfp4_tile_scales(rows[1]).view(torch.uint8), tiles.view(torch.uint8))
+    back = P.nvfp4_dequantize(codes, rows[1], g, torch.float32)
+    blocks, got = w.double().view(3, 64, 16, 16), back.double().view(3, 64, 16, 16)
+    amax = blocks.abs().amax(-1, keepdim=True)
+    bad = ~amax.isfinite().expand_as(got)
+    assert torch.equal(got.isnan(), bad) and int(bad.sum()) == 3 * 16
+    # (1/6 of amax and 2^-4, float32's rounding of subnormal products: 2^-149)
+    bound = amax * (1 / 6 + 2.0 ** -4) * (1 + 2.0 ** -20) + 6 * g.double().view(3, 1, 1, 1) * 2.0 ** -10 + 2.0 ** -149
+    assert ((got - blocks).abs() <= bound)[~bad].all()
+
+
 # ---- permute ----------------------------------------------------------------------
 
 

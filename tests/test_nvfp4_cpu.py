@@ -187,6 +187,27 @@ def test_tile_scales_refusals():
         P.nvfp4_quantize_weights(torch.zeros(4, 64, dtype=torch.bfloat16))
 
 
+def test_weight_global_scales():
+    """The largest finite magnitude over 2688, 1 for zeros, at least 2^-100."""
+    from layerstormexpertkernels_b200.nvfp4 import weight_global_scales
+    w = torch.zeros(8, 4, 32, dtype=torch.bfloat16)
+    w[0, 1, 5] = -3.0
+    w[1, 2, 7], w[1, 0, 0] = 0.25, float("inf")
+    w[2, 2, 7], w[2, 0, 0], w[2, 1, 1] = 0.25, float("nan"), -float("inf")
+    w[3, 0, 0] = float("nan")
+    w[4, 0, 3] = 2.0 ** -133   # the smallest bf16
+    w[5, 0, 3] = 2.0 ** -95
+    w[6, 3, 3] = torch.finfo(torch.bfloat16).max
+    got = weight_global_scales(w).double()
+    low = 2.0 ** -100
+    want = torch.tensor([3 / 2688, 0.25 / 2688, 0.25 / 2688, 1.0, low, low,
+                         torch.finfo(torch.bfloat16).max / 2688, 1.0], dtype=torch.float64)
+    assert ((got - want).abs() <= want * 2.0 ** -24).all()
+    assert w[1, 0, 0].isinf() and w[2, 0, 0].isnan()  # the weights stay as they are
+    assert float(got[6]) < 2.0 ** 117
+    assert weight_global_scales(w[:0]).shape == (0,) and (weight_global_scales(w[:, :0]) == 1).all()
+
+
 def test_oracle_quantiser_is_nearest():
     """The oracle's codes against a search over all codes in 64 bits, away from
     the borders, and the ties on exact borders with a power-of-two scale."""
