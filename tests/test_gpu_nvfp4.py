@@ -444,6 +444,59 @@ def test_swiglu_equals_product_swiglu_quantize(counts, inter, k, limit):
     assert (err <= amax * (1 / 6 + 2.0 ** -4 + 2.0 ** -7 + 1e-3) + smallest).all()
 
 
+def same_as_three_operators(counts, inter, k, limit, seed, runs):
+    """The fused kernel, `runs` times, against product + fused_swiglu + quantise."""
+    P = pk()
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(sum(counts), k, generator=gen, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(len(counts), 2 * inter, k, generator=gen, device="cuda") * (2.0 / np.sqrt(k))).to(torch.bfloat16)
+    off = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device="cuda")
+    ga, go = glob(0.01), glob(0.02)
+    a, asf = P.nvfp4_quantize(x, ga)
+    wc, wt, gw = P.nvfp4_quantize_weights(w, 2)
+    got = [P.grouped_gemm_swiglu_nvfp4(a, asf, wc, wt, off, ga, gw, go, swiglu_limit=limit) for _ in range(runs)]
+    one = P.nvfp4_tile_scales(P.nvfp4_quantize(w, gw)[1], 1)
+    gu = P.grouped_gemm_nvfp4(a, asf, wc, one, off, ga, gw)
+    want, want_s = P.nvfp4_quantize(P.fused_swiglu(gu, swiglu_limit=limit), go)
+    sync_and_check_device_error()
+    for h, hs in got:
+        assert torch.equal(hs.view(torch.uint8), want_s.view(torch.uint8)) and torch.equal(h, want)
+    return a, asf, w, gu, ga
+
+
+@pytest.mark.parametrize("counts,inter,k,limit", [
+    ([8] * 160, 160, 256, 0.0),                                            # one short unit after another
+    ([95, 96, 97, 191, 192, 193, 0, 400, 1, 1000, 17, 33], 2048, 1088, 10.0),  # one and two accumulators, mixed
+    ([700, 30, 811, 5, 640, 97] * 3, 1056, 2304, 0.0),
+    ([1024, 300, 1500, 90, 2000, 64, 700, 1300], 2048, 7168, 0.0),         # full load
+])
+def test_swiglu_of_many_units_a_block(counts, inter, k, limit):
+    """Several units for each block, so that accumulators, turning buffers and
+    ring slots are used again: four runs with the bits of the three operators."""
+    units = sum(-(-c // 192) for c in counts) * -(-inter // 128)
+    assert units > 2 * 148
+    a, asf, w, gu, ga = same_as_three_operators(counts, inter, k, limit, seed=len(counts) + k, runs=4)
+    # and g, u against 64-bit sums, for the largest expert
+    e = int(np.argmax(counts))
+    lo = sum(counts[:e])
+    P = pk()
+    rows = P.nvfp4_dequantize(a[lo:lo + counts[e]], asf[lo:lo + counts[e]], None, torch.float32).double()
+    we = w[e:e + 1].contiguous()
+    wc, _, gw = P.nvfp4_quantize_weights(we, 2)
+    wv = P.nvfp4_dequantize(wc, P.nvfp4_quantize(we, gw)[1], None, torch.float32)[0].double()
+    alpha = ga.double() * gw.double()
+    exact, mag = alpha * (rows @ wv.T), alpha * (rows.abs() @ wv.abs().T)
+    acc = (k / 64 + 8 + 2) * 2.0 ** -23 * mag
+    assert ((gu[lo:lo + counts[e]].double() - exact).abs() <= acc + 2.0 ** -8 * (exact.abs() + acc)).all()
+
+
+def test_swiglu_of_more_than_256_experts():
+    gen = torch.Generator().manual_seed(14)
+    counts = [int(c) for c in torch.randint(0, 4, (300,), generator=gen)]
+    counts[7], counts[299], counts[150] = 210, 97, 400
+    same_as_three_operators(counts, 160, 320, 0.0, seed=15, runs=3)
+
+
 def test_swiglu_for_every_gate_value():
     """Every bf16 gate magnitude and sign from 2^-126 up (128 significands as
     columns, 18 exponents and both signs as tokens, 15 experts for the rest of
@@ -782,6 +835,40 @@ def test_layer_equals_its_operators(T, E, H, I, k, ng, tg, limit):
         hidden_global_scale=layer.hidden_global_scale, inter_global_scale=layer.inter_global_scale,
         return_routing=True)
     assert torch.equal(fn[0], want) and torch.equal(fn[2], idx)
+
+
+@pytest.mark.parametrize("T,E,H,I,k,ng,tg", [
+    (300, 16, 2560, 2048, 4, 4, 2),
+    (2100, 8, 2560, 2112, 2, 1, 1),
+    (90, 320, 1536, 256, 8, 8, 4),      # more than 256 experts
+    (1500, 320, 512, 128, 8, 1, 1),
+])
+def test_layer_of_many_units_on_a_dirty_workspace(T, E, H, I, k, ng, tg):
+    """Both products have more units than blocks, so they share them out by the
+    counters that the row copy zeroes: right on a workspace full of ones, on one
+    that holds the counts of the call before, and at each replay of a graph."""
+    units = [(T * k // 192 + min(E, T * k)) * n for n in (-(-I // 128), -(-H // 256))]
+    assert min(units) > 148 and T * k > 192
+    layer, x, logits = make_layer(T, E, H, I, k, ng, tg, seed=T + E)
+    want = by_operators(layer, x, logits)[0]
+    layer._ensure_workspace(T)
+    layer.workspace.fill_(0xFF)
+    assert torch.equal(layer(x, logits), want)
+    assert torch.equal(layer(x, logits), want)
+    out = torch.empty_like(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        layer(x, logits, out=out)
+    for rep in range(3):
+        if rep == 2:
+            x.copy_(x.flip(0))
+            want = by_operators(layer, x, logits)[0]
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), rep
+    sync_and_check_device_error()
 
 
 def test_layer_close_to_the_bf16_layer():
