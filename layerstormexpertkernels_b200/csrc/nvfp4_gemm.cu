@@ -315,8 +315,9 @@ __device__ __forceinline__ uint32_t fp4_idesc(int nn) {
 // flush-to-zero forms of the exponential and the reciprocal: half its
 // instructions, which bound this epilogue.  Results that are bf16 subnormals
 // may come out as zeros of the same sign, which quantise to the same codes
-// (their quotients are below 2^-17); all others have swiglu_f32's bits, tried for
-// every bf16 g.
+// (their quotients are below 2^-17); the others have swiglu_f32's bits.  Tests
+// compare the bits of h for every bf16 g from 2^-126 up, of both signs, with up
+// values of three exponents, and the codes behind them.
 template <bool CLAMP>
 __device__ __forceinline__ void swiglu_turn(const uint32_t (&g2)[8], const uint32_t (&u2)[8],
                                             float limit, uint8_t* turn, int lane) {

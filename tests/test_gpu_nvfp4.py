@@ -537,6 +537,66 @@ def test_swiglu_for_every_gate_value():
     sync_and_check_device_error()
 
 
+@pytest.mark.parametrize("limit", [0.0, 10.0])
+def test_swiglu_has_every_bit_of_fused_swiglu(limit):
+    """The fused kernel's h to the last bf16 bit, which its 4-bit outputs hide: a
+    block has one value other than 0, so its scale is e4m3(|h| / (6 go)), and go
+    goes through an eighth of an octave in steps of 0.35 %, finer than a bf16 step
+    (0.39 % at least): for one of them a border of two scales lies between h and
+    its neighbour.  (The same sweep with h one step up has to show it for every h
+    of normal size.)  Gates: every bf16 magnitude from 2^-126 up and both signs;
+    up values with other significands and with exponents of 9 below to 8 above
+    the gate's range."""
+    P = pk()
+    inter, k, E = 2048, 256, 15
+    b = torch.arange(128)
+    w = torch.zeros(2 * inter, k // 16)  # rows 16 b: bit i of a significand at block i (gate) or 8 + i (up)
+    for i in range(8):
+        w[16 * b, i] = (((128 + b) >> i) & 1) * 2.0 ** i
+        w[inter + 16 * b, 8 + i] = (((128 + 37 * b % 128) >> i) & 1) * 2.0 ** i
+    codes = torch.zeros(2 * inter, k // 2, dtype=torch.uint8)
+    codes[:, ::8] = 2  # 1.0 at the first element of each block
+    signs, exps, ups = torch.tensor([2, 10]), torch.arange(-9, 9), torch.tensor([-9, 0, 8])
+    n = len(signs) * len(exps) * len(ups)
+    grid = torch.cartesian_prod(signs, exps, ups)
+    tokens = torch.zeros(n, k // 2, dtype=torch.uint8)
+    tokens[:, :64:8] = grid[:, :1].to(torch.uint8)
+    tokens[:, 64::8] = 2
+    ascale = torch.exp2(torch.cat([grid[:, 1:2].expand(n, 8), grid[:, 2:3].expand(n, 8)], 1).float())
+    off = torch.arange(E + 1, dtype=torch.int32, device="cuda") * n
+    gw = torch.exp2(torch.arange(E).float() * 18 - 124).cuda()
+    a = tokens.repeat(E, 1).cuda()
+    asf = ascale.repeat(E, 1).to(torch.float8_e4m3fn).cuda()
+    wc = codes[None].repeat(E, 1, 1).cuda()
+    wsf = w[None].repeat(E, 1, 1).to(torch.float8_e4m3fn).cuda()
+    two, one = P.nvfp4_tile_scales(wsf, 2), P.nvfp4_tile_scales(wsf, 1)
+    gu = P.grouped_gemm_nvfp4(a, asf, wc, one, off, None, gw)
+    g = gu[:, :inter:16].float()
+    assert g[g.isfinite()].abs().unique().numel() > 128 * 250
+    h = P.fused_swiglu(gu, swiglu_limit=limit)
+    # (2^128 is infinite in float32: the last expert's blocks are NaN)
+    assert (h[:14 * n, 1::16] == 0).all()
+    bits = h[:, ::16].contiguous().view(torch.int16)
+    up = h.clone()
+    up[:, ::16] = (bits + (bits & 0x7FFF < 0x7F7F).short()).view(torch.bfloat16)  # one step up, none past the largest
+    shown = torch.zeros(g.shape, dtype=torch.bool, device="cuda")
+    for e in range(-100, 101, 14):
+        for i in range(36):
+            go = glob(2.0 ** e * (1 + 0.0035 * i))
+            got, got_s = P.grouped_gemm_swiglu_nvfp4(a, asf, wc, two, off, None, gw, go, swiglu_limit=limit)
+            want, want_s = P.nvfp4_quantize(h, go)
+            assert torch.equal(got_s.view(torch.uint8), want_s.view(torch.uint8)), (e, i)
+            assert torch.equal(got, want), (e, i)
+            shown |= P.nvfp4_quantize(up, go)[1].view(torch.uint8) != want_s.view(torch.uint8)
+    size = h[:, ::16].float().abs()
+    # within the scales' normal range of some go (2^-6 to 448, 6 go = 2^-97.4 to 2^96.6)
+    normal = (size > 2.0 ** -103) & (size < 2.0 ** 105)
+    normal[14 * n:] = False
+    # by the formula in 64 bits 62908 of h without and 90864 with the clamp lie there
+    assert normal.sum() > (90_000 if limit else 62_000) and shown[normal].all()
+    sync_and_check_device_error()
+
+
 def test_swiglu_clamp_keeps_nan():
     """A token with NaN among its values is NaN in every block behind the
     clamped gate/up kernel and behind the layer, and the other tokens are as
