@@ -286,7 +286,8 @@ LSEK_API lsek_status lsek_grouped_gemm_swiglu_bf16(void* Hout, const void* A,
  * 16 elements, every operation rounded to float32 once:
  *   scale = e4m3(amax / (6 * global_scale))       saturating at 448
  *   code  = e2m1(x * (1 / (scale * global_scale))) saturating at 6
- * (nearest, halves to even; codes 0 where the scale is 0).  A block that
+ * (nearest, halves to even; where the scale is 0, x * 0: codes 0, and 8 for
+ * negative x).  A block that
  * holds an infinity or a NaN gets the scale NaN.  k % 16 == 0; global scales
  * are positive, in [2^-100, 2^117]; codes 8-byte aligned. */
 LSEK_API lsek_status lsek_nvfp4_quantize(void* codes, void* scales, const void* x,

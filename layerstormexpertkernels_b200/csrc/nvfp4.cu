@@ -3,16 +3,16 @@
 // All three are HBM streams: the quantiser reads 2 bytes and writes 0.5625
 // bytes an element, the dequantiser the reverse, and the permute reads each
 // token once and writes 0.5625 bytes an element to each of its topk rows.
-// One thread takes a block of 16 elements at a time: 32 bytes in (one access),
-// 8 bytes of codes and one scale byte out, so a warp reads 1 KB and writes
-// 256 + 32 bytes, all contiguous.  Blocks do not cross rows (the row length is
-// a multiple of 16), so a contiguous tensor is one flat run of blocks.
+// A thread's access is a block of 16 elements: 32 bytes in (one access), 8 bytes
+// of codes and one scale byte out, so a warp reads 1 KB and writes 256 + 32
+// bytes, all contiguous; the quantiser and the dequantiser have four blocks in
+// flight a thread.  Blocks do not cross rows (the row length is a multiple of
+// 16), so a contiguous tensor is one flat run of blocks.  At 16 x 4096 x 7168
+// each of the two takes 184 us, 6.5 TB/s; to fp32 (four 16-byte stores 64 bytes
+// apart) the dequantiser takes 497 us, 4.3 TB/s.
 #include "nvfp4.cuh"
 
 namespace lsek {
-
-lsek_status launch_route_by_expert(const int32_t* idx, int64_t n, int E, int32_t* offsets,
-                                   int32_t* s2d, int32_t* perm, cudaStream_t st);  // permute.cu
 
 namespace {
 

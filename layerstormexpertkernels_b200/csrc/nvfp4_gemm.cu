@@ -33,17 +33,21 @@
 // that start at any expert boundary, from there too where TMA can load them
 // (K % 256 == 0: rows of whole 16-byte pieces) and from global memory
 // otherwise.  (Loading them from global memory always costs 45 to 70 % more
-// time at 128 to 1024 rows an expert: 32 lines a load, in four warps.)  Copying
-// the weights' tiles with tcgen05.cp from the MMA warp instead is 1 to 9 % slower
-// (down product, 16 experts of 1024 rows: 171 against 156 us): eight more
-// instructions a stage in the lane that paces the MMAs.
+// time at 128 to 1024 rows an expert: 32 lines a load, in four warps.  So a K
+// that is no multiple of 256 costs: N=4096, K=2112 against 2304 takes 39 and 37
+// us at 32 experts x 16 rows, 50 and 45 at 32 x 128, 124 and 102 at 16 x 1024.)
+// Copying the weights' tiles with tcgen05.cp from the MMA warp instead is 1 to
+// 9 % slower (down product, 16 experts of 1024 rows: 171 against 156 us): eight
+// more instructions a stage in the lane that paces the MMAs.
 //
 // Bounds, measured on a B200 with 64 experts, H=7168, I=2048 (6.54 TB/s copy):
 // up to 64 rows an expert the weights' stream, gate/up 163 to 167 us = 6.5 to 6.3
 // TB/s; at 128 rows 190 us = 5.6 TB/s, where a tile takes both accumulators and
 // its epilogue's first part stands between two main loops; at 1024 rows (16
-// experts) 241 us = 4.0 PFLOP/s, bound by the loads into shared memory (64 KB a
-// stage of about 900 cycles) and that same gap.
+// experts) 239 us = 4.0 PFLOP/s in a burst and 279 us = 3.5 PFLOP/s in a long run,
+// where the power cap holds the SM clock at 1492 MHz.  That is 291 stages of 62
+// KB for an SM, 0.82 and 0.96 us (1430 cycles) each with the gaps between main
+// loops counted in: bound by the loads into shared memory and those gaps.
 //
 // One CTA = 16 warps:
 //   warp 0       takes units; TMA producer of the weights' codes
