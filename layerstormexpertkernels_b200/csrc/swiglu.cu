@@ -9,12 +9,15 @@
 namespace lsek {
 namespace {
 
-template <typename T>
+template <typename T, bool CLAMP>
 __global__ void __launch_bounds__(256) swiglu_vec_kernel(T* __restrict__ out,
                                                          const T* __restrict__ in, int64_t N,
                                                          int d, float limit) {
   const int vpr = d / 8;
   const int64_t total = N * vpr;
+  // Not unrolled: most threads take one step (unrolled, 4096 x 2048 took 12.3 us
+  // instead of 10.3).
+#pragma unroll 1
   for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t n = i / vpr;
@@ -26,21 +29,11 @@ __global__ void __launch_bounds__(256) swiglu_vec_kernel(T* __restrict__ out,
     const T* ue = reinterpret_cast<const T*>(&uraw);
     uint4 oraw;
     T* oe = reinterpret_cast<T*>(&oraw);
-    float gf[8], uf[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      gf[j] = Elem<T>::to_f(ge[j]);
-      uf[j] = Elem<T>::to_f(ue[j]);
+      const float gf = Elem<T>::to_f(ge[j]), uf = Elem<T>::to_f(ue[j]);
+      oe[j] = Elem<T>::from_f(CLAMP ? swiglu_f32(gf, uf, limit) : silu_mul(gf, uf));
     }
-    if (limit > 0.0f) {  // one branch for the eight
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        gf[j] = clamp_gate(gf[j], limit);
-        uf[j] = clamp_up(uf[j], limit);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) oe[j] = Elem<T>::from_f(silu_mul(gf[j], uf[j]));
     *reinterpret_cast<uint4*>(out + n * d + static_cast<int64_t>(v) * 8) = oraw;
   }
 }
@@ -71,8 +64,9 @@ lsek_status launch_swiglu_t(void* out, const void* in, int64_t N, int d, float l
   const int64_t cap = 32ll * num_sms();
   if (grid > cap) grid = cap;
   if (vec_ok)
-    swiglu_vec_kernel<T><<<static_cast<unsigned>(grid), threads, 0, st>>>(
-        static_cast<T*>(out), static_cast<const T*>(in), N, d, limit);
+    (limit > 0.0f ? swiglu_vec_kernel<T, true> : swiglu_vec_kernel<T, false>)<<<
+        static_cast<unsigned>(grid), threads, 0, st>>>(static_cast<T*>(out),
+                                                       static_cast<const T*>(in), N, d, limit);
   else
     swiglu_scalar_kernel<T><<<static_cast<unsigned>(grid), threads, 0, st>>>(
         static_cast<T*>(out), static_cast<const T*>(in), N, d, limit);

@@ -9,8 +9,7 @@ namespace lsek {
 // The clamp of ref_swiglu (tests/test_reference.py:110-125): g = min(g, L),
 // u = clamp(u, -L, L), L > 0.  NaN stays NaN, as in torch.clamp, so that it is
 // seen downstream; fminf and fmaxf would return the limit for it.  The second
-// is one instruction: the smaller of |u| and L with the sign of u (as a maximum
-// and a minimum it took 3 % of fused_swiglu's time at 65536 x 2048).
+// is one instruction: the smaller of |u| and L with the sign of u.
 __device__ __forceinline__ float clamp_gate(float g, float limit) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(g), "f"(limit));
