@@ -376,6 +376,74 @@ def test_rows_behind_the_last_expert_stay():
         assert_product(d[:230], av, wv, off, [1.0] * 3)
 
 
+@pytest.mark.parametrize("scratch", [0, 3, 4])
+def test_many_units_without_a_counter(scratch):
+    """The C ABI without scratch, and with less than a counter needs, shares units
+    out by a fixed stride; with 4 bytes by the counter, whatever they hold: the
+    bits of the binding's call, through both products.  The first expert starts
+    behind 13 rows that belong to none and stay as they were, like those behind
+    the last."""
+    P = pk()
+    counts, n, k = [300, 5, 0, 700, 190, 193, 60] * 5, 1024, 512
+    a, asf, av, w, tiles, wv, off, _ = make_product(counts, n, k, seed=61, pad_rows=30)
+    d_off = torch.tensor([o + 13 for o in off], dtype=torch.int32, device="cuda")
+    rows, lo, hi = a.shape[0], 13, 13 + off[-1]
+    lib = ctypes.CDLL(P.LIBRARY_PATH)
+    ptr = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    ws = torch.full((256,), 0xFF, dtype=torch.uint8, device="cuda")
+    tail = (ptr(ws) if scratch else None, ctypes.c_size_t(scratch), stream)
+    gate = P.nvfp4_tile_scales(rand_fp4(torch.Generator().manual_seed(62), len(counts), n, k)[1], 2)
+    go = glob(8.0)
+    d = torch.full((rows, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    h = torch.full((rows, n // 4), 0xAB, dtype=torch.uint8, device="cuda")
+    hs = torch.full((rows, n // 32), 0xAB, dtype=torch.uint8, device="cuda")
+    assert lib.lsek_grouped_gemm_nvfp4(ptr(d), ptr(a), ptr(asf), ptr(w), ptr(tiles), ptr(d_off), None, None,
+                                       len(counts), rows, n, k, *tail) == 0
+    assert lib.lsek_grouped_gemm_swiglu_nvfp4(ptr(h), ptr(hs), ptr(a), ptr(asf), ptr(w), ptr(gate), ptr(d_off),
+                                              None, None, ptr(go), len(counts), rows, n // 2, k,
+                                              ctypes.c_float(0.0), *tail) == 0
+    sync_and_check_device_error()
+    want = P.grouped_gemm_nvfp4(a, asf, w, tiles, d_off)
+    want_h, want_hs = P.grouped_gemm_swiglu_nvfp4(a, asf, w, gate, d_off, None, None, go)
+    sync_and_check_device_error()
+    for got, ref, old in ((d, want, 7.0), (h, want_h, 0xAB), (hs, want_hs.view(torch.uint8), 0xAB)):
+        assert torch.equal(got[lo:hi], ref[lo:hi])
+        assert (got[:lo] == old).all() and (got[hi:] == old).all()
+    assert_product(d[lo:hi], av[lo:hi], wv, off, [1.0] * len(counts))
+
+
+def test_products_captured_and_replayed():
+    """A graph of gate/up and down product with more units than blocks: every
+    replay zeroes its counters, and takes the inputs of the moment."""
+    P = pk()
+    counts, k = [300, 5, 0, 700, 190, 193, 60, 250], 1024
+    gen = torch.Generator(device="cuda").manual_seed(71)
+    x = torch.randn(sum(counts), k, generator=gen, device="cuda").to(torch.bfloat16)
+    off = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32, device="cuda")
+    gu, gut, gug = P.nvfp4_quantize_weights(torch.randn(8, 2 * 2048, k, generator=gen, device="cuda").to(torch.bfloat16), 2)
+    dn, dnt, dng = P.nvfp4_quantize_weights(torch.randn(8, 5120, 2048, generator=gen, device="cuda").to(torch.bfloat16))
+    ga, gh = glob(0.01), glob(300.0)
+
+    def run():
+        a, asf = P.nvfp4_quantize(x, ga)
+        h, hs = P.grouped_gemm_swiglu_nvfp4(a, asf, gu, gut, off, ga, gug, gh)
+        return h, hs, P.grouped_gemm_nvfp4(h, hs, dn, dnt, off, gh, dng)
+
+    run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for rep in range(3):
+        x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        g.replay()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(got, run()))
+    sync_and_check_device_error()
+
+
 def test_nan_scale_reaches_only_its_row():
     """A block with a NaN scale (a non-finite activation) makes its token's
     outputs NaN and leaves the others as they were."""
